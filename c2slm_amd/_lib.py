@@ -17,6 +17,9 @@ LIB_PATH = os.environ.get("C2H_LIB") or os.path.join(HERE, "libc2h.so")
 C2H_OK = 0
 NOALLOC_MAX_COLS = 16384  # C2H_NOALLOC_MAX_COLS
 F32, Q5_0, Q8_0, Q4_K, Q6_K = 0, 6, 8, 12, 14
+F16, BF16, F8_E4M3 = 1, 30, 100  # activations and paged caches
+ROPE_LAYOUT = dict(half=0, interleaved=1)  # C2H_ROPE_*
+ROPE_MAX_DIM = 256
 
 ROLE = dict(TOKEN_EMBD=0, OUTPUT=1, OUTPUT_NORM=2, ATTN_NORM=10, ATTN_Q=11, ATTN_Q_BIAS=12, ATTN_K=13,
             ATTN_K_BIAS=14, ATTN_V=15, ATTN_V_BIAS=16, ATTN_OUT=17, FFN_NORM=18, FFN_GATE=19, FFN_UP=20,
@@ -35,6 +38,37 @@ class ModelDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n_layers", "n_embd", "n_heads", "n_kv_heads", "head_dim", "n_ff",
                                          "n_vocab", "max_ctx")] + \
                [("rms_eps", C.c_float), ("rope_theta", C.c_float), ("reserved", C.c_int32 * 6)]
+
+
+class Heads(C.Structure):
+    """c2h_heads: head vectors of a run of tokens in device memory."""
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [("rot_dim", C.c_int32), ("layout", C.c_int32), ("base", C.c_double), ("mscale", C.c_double),
+                ("factor", C.c_double), ("orig_ctx", C.c_int32), ("reserved", C.c_int32), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("freq_factors", C.c_void_p)]
+
+
+class Rope(C.Structure):
+    """c2h_rope: a rotation that rope() filled."""
+    _fields_ = [("rot_dim", C.c_int32), ("layout", C.c_int32), ("mscale", C.c_float), ("reserved", C.c_int32),
+                ("turns", C.c_double * (ROPE_MAX_DIM // 2))]
+
+
+class PagedKV(C.Structure):
+    """c2h_paged_kv: a pool of pages of keys and values."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_int32) for n in ("type", "n_pages", "page_size", "n_kv_heads", "head_dim", "reserved")] + \
+               [(n, C.c_int64) for n in ("page_stride", "token_stride", "head_stride")] + \
+               [("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class PagedBatch(C.Structure):
+    """c2h_paged_batch: the sessions of a call and their pages."""
+    _fields_ = [("block_table", C.c_void_p), ("table_stride", C.c_int64), ("seq_lens", C.c_void_p),
+                ("n_seqs", C.c_int32), ("max_len", C.c_int32)]
 
 
 class C2hError(RuntimeError):
@@ -97,6 +131,17 @@ def lib():
             "c2h_gemv_f32_dev": (C.c_int, [VP, I32, VP, VP, I32, I32, VP]),
             "c2h_logits_ids": (C.c_int, [VP, VP, I32, VP]),
             "c2h_logits_ids_dev": (C.c_int, [VP, VP, I32, VP]),
+            "c2h_rope_init": (C.c_int, [C.POINTER(RopeDesc), C.POINTER(Rope)]),
+            "c2h_rope_dev": (C.c_int, [VP, C.POINTER(Rope), I32, C.POINTER(Heads), VP, I32, I32, I32,
+                                       C.POINTER(Heads)]),
+            "c2h_paged_append_dev": (C.c_int, [VP, C.POINTER(PagedKV), C.POINTER(PagedBatch), VP, I32, C.POINTER(Rope),
+                                               I32, C.POINTER(Heads), C.POINTER(Heads), I32, C.POINTER(Heads),
+                                               C.POINTER(Heads)]),
+            "c2h_paged_attn_dev": (C.c_int, [VP, C.POINTER(PagedKV), C.POINTER(PagedBatch), I32, I32, C.c_float, I32,
+                                             C.POINTER(Heads), C.POINTER(Heads)]),
+            "c2h_paged_attn_workspace": (C.c_int, [C.POINTER(PagedKV), C.POINTER(PagedBatch), I32, I32,
+                                                   C.POINTER(C.c_size_t)]),
+            "c2h_rmsnorm_q8k_dev": (C.c_int, [VP, I32, VP, I64, VP, I64, VP, C.c_float, I32, I32, VP, I64, VP, VP, I64]),
             "c2h_time_dot_rows": (C.c_int, [VP, I32, VP, VP, I32, I32, VP, I32, I32, C.c_int64, VP,
                                             C.POINTER(C.c_float)]),
         }
@@ -343,6 +388,93 @@ class Ctx:
         y = np.empty(rows, np.float32)
         self._chk(lib().c2h_gemv_f32(self.h, ggml_type, _p(w), _p(x), rows, cols, _p(y)))
         return y
+
+
+    # ---- operators for many sessions (device memory; asynchronous: sync() waits)
+    #
+    # Tensors are objects with data_ptr(), stride() and shape (torch's), on
+    # the context's GPU and complete; they must live until the work is done.
+    def rope_dev(self, rope: Rope, ggml_type: int, x: Heads, positions, n_tokens: int, n_heads: int, head_dim: int,
+                 y: Heads):
+        """y = x rotated to positions (c2h_rope_dev)."""
+        self._chk(lib().c2h_rope_dev(self.h, rope, ggml_type, x, _dp(positions), n_tokens, n_heads, head_dim, y))
+
+    def paged_append_dev(self, kv: PagedKV, batch: PagedBatch, ggml_type: int, n_tokens: int, k: Heads, v: Heads,
+                         token_start=None, rope: Rope | None = None, q: Heads | None = None, q_out: Heads | None = None,
+                         n_heads: int = 0):
+        """Keys and values of new tokens into their pages, K rotated, and the
+        queries rotated to q_out (c2h_paged_append_dev)."""
+        self._chk(lib().c2h_paged_append_dev(self.h, kv, batch, _dp(token_start), n_tokens, rope, ggml_type, k, v,
+                                             n_heads, q, q_out))
+
+    def paged_attn_dev(self, kv: PagedKV, batch: PagedBatch, ggml_type: int, n_heads: int, scale: float, q: Heads,
+                       out: Heads, window: int = 0):
+        """One new token per session over its pages (c2h_paged_attn_dev)."""
+        self._chk(lib().c2h_paged_attn_dev(self.h, kv, batch, ggml_type, n_heads, scale, window, q, out))
+
+    def rmsnorm_q8k_dev(self, ggml_type: int, x, w, eps: float, q8k, residual=None, sum_out=None, y=None):
+        """Rows of x (plus residual, to sum_out) normalised, times w, to Q8_K
+        rows and, where y is given, floats (c2h_rmsnorm_q8k_dev)."""
+        self._chk(lib().c2h_rmsnorm_q8k_dev(
+            self.h, ggml_type, x.data_ptr(), x.stride(0), _dp(residual), residual.stride(0) if residual is not None else 0,
+            w.data_ptr(), eps, x.shape[0], x.shape[1], _dp(sum_out), sum_out.stride(0) if sum_out is not None else 0,
+            q8k.data_ptr(), _dp(y), y.stride(0) if y is not None else 0))
+
+
+def _dp(t):
+    return None if t is None else t.data_ptr()
+
+
+def heads(t) -> Heads:
+    """A tensor [tokens, heads, head_dim] as c2h_heads (its strides as they
+    are; elements of a head contiguous)."""
+    if t.ndim != 3 or t.stride(2) != 1:
+        raise ValueError("heads() takes [tokens, heads, head_dim] with contiguous elements")
+    return Heads(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def rope(rot_dim: int, base: float, layout: str = "half", factor: float = 1.0, orig_ctx: int = 0,
+         beta_fast: float = 32.0, beta_slow: float = 1.0, mscale: float = 1.0, freq_factors=None) -> Rope:
+    """A rotation for rope_dev and paged_append_dev (c2h_rope_init)."""
+    f = None if freq_factors is None else np.ascontiguousarray(freq_factors, dtype=np.float32)
+    if f is not None and len(f) != rot_dim // 2:
+        raise ValueError("freq_factors: one per pair")
+    d = RopeDesc(rot_dim, ROPE_LAYOUT[layout], base, mscale, factor, orig_ctx, 0, beta_fast, beta_slow,
+                 None if f is None else f.ctypes.data)
+    r = Rope()
+    rc = lib().c2h_rope_init(C.byref(d), C.byref(r))
+    if rc != C2H_OK:
+        raise C2hError(rc, (lib().c2h_last_error(None) or b"").decode())
+    return r
+
+
+def paged_kv(k, v, ggml_type: int, order: str = "nhd", k_scale=None, v_scale=None) -> PagedKV:
+    """Pools k and v as c2h_paged_kv: tensors [pages, page_size, kv_heads,
+    head_dim] (order "nhd") or [pages, kv_heads, page_size, head_dim]
+    ("hnd") of equal strides; k_scale and v_scale: kv_heads floats on the GPU."""
+    if k.shape != v.shape or k.stride() != v.stride() or k.ndim != 4 or k.stride(3) != 1:
+        raise ValueError("paged_kv() takes two pools of four dimensions, of equal shapes and strides")
+    t, h = (1, 2) if order == "nhd" else (2, 1)
+    return PagedKV(k.data_ptr(), v.data_ptr(), ggml_type, k.shape[0], k.shape[t], k.shape[h], k.shape[3], 0, k.stride(0),
+                   k.stride(t), k.stride(h), _dp(k_scale), _dp(v_scale))
+
+
+def paged_batch(block_table, seq_lens, max_len: int) -> PagedBatch:
+    """Sessions as c2h_paged_batch: int32 tensors [sessions, pages] and
+    [sessions] on the GPU, and a bound of the lengths."""
+    if block_table.ndim != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0]:
+        raise ValueError("paged_batch() takes a table [sessions, pages] and as many lengths")
+    return PagedBatch(block_table.data_ptr(), block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
+                      seq_lens.data_ptr(), seq_lens.shape[0], max_len)
+
+
+def paged_attn_workspace(kv: PagedKV, batch: PagedBatch, n_heads: int, window: int = 0) -> int:
+    """Bytes of the context's workspace that paged_attn_dev takes."""
+    n = C.c_size_t()
+    rc = lib().c2h_paged_attn_workspace(C.byref(kv), C.byref(batch), n_heads, window, C.byref(n))
+    if rc != C2H_OK:
+        raise C2hError(rc, (lib().c2h_last_error(None) or b"").decode())
+    return n.value
 
 
 def packed_size(ggml_type: int, rows: int, cols: int) -> int:

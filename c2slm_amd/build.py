@@ -21,7 +21,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libc2h.so")
 ARCH = os.environ.get("C2H_OFFLOAD_ARCH", "gfx950")
 
-SOURCES = ["c2h_kernels.hip", "c2h_api.hip"]
+SOURCES = ["c2h_kernels.hip", "c2h_paged.hip", "c2h_api.hip"]
 
 
 def hipcc() -> str:

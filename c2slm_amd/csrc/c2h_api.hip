@@ -16,6 +16,7 @@
 #include "../../include/c2h.h"
 #include "c2h_device.h"
 #include "c2h_kernels.h"
+#include "c2h_paged.h"
 
 using namespace c2h;
 
@@ -75,7 +76,9 @@ struct c2h_ctx {
   float* logits = nullptr;
   C2hState* state_dev = nullptr;
   C2hState* state_ring = nullptr;  // pinned
-  int32_t* tok_host = nullptr;     // pinned: {token, seq} written by a step's layer 0; [2] the wait flag
+  // pinned: {token, seq} written by a step's layer 0; [2] the wait flag; [3]
+  // what the operators on paged caches found wrong (PagedErr)
+  int32_t* tok_host = nullptr;
   unsigned step_seq = 0;           // last step number handed to the device
   // the state a completed step graph leaves on the device (its final norm
   // advances pos, seq and the normX buffers); valid until the next push
@@ -119,6 +122,9 @@ struct c2h_ctx {
   bool dot_attr = false;  // k_dot_rows LDS limit raised
   uint8_t* vq8k = nullptr;  // Q8_K row of normX for a K-quant output.weight
   uint8_t* noalloc = nullptr;  // this device's copy of `scratch` (c2h_quantize_q8k_noalloc)
+  // partial rows of c2h_paged_attn_dev (grown by the call that needs more)
+  float* paged_ws = nullptr;
+  size_t paged_ws_bytes = 0;
 };
 
 // Device scratch of c2h_quantize_q8k_noalloc, which calls no allocator:
@@ -133,13 +139,15 @@ static __device__ __align__(256) uint8_t scratch[kNoAllocX + kNoAllocY];
 
 namespace {
 
+thread_local std::string g_create_err;  // c2h_last_error(NULL)
+
 int fail(c2h_ctx* c, int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
-  if (c) c->err = buf;
+  (c ? c->err : g_create_err) = buf;
   return code;
 }
 
@@ -1220,6 +1228,15 @@ int check_wait_flag(c2h_ctx* c) {
   return fail(c, C2H_ERR_HIP, "a wait for the attention output inside a launch ran out");
 }
 
+// The same for what the operators on paged caches found in tables and lengths.
+int check_paged_flag(c2h_ctx* c) {
+  const int what = c->tok_host ? __atomic_exchange_n(&c->tok_host[3], 0, __ATOMIC_ACQ_REL) : 0;
+  if (what == 0) return C2H_OK;
+  return fail(c, C2H_ERR_RANGE, "paged batch:%s%s%s", what & PERR_LENGTH ? " a length outside [0, max_len];" : "",
+              what & PERR_PAGE ? " a page index outside the pool;" : "",
+              what & PERR_START ? " more new tokens than the session holds;" : "");
+}
+
 // Decode at `pos` attends to pos+1 positions.
 int run_graph(c2h_ctx* c, bool step, int pos) {
   const int form = attn_form(c, pos + 1);
@@ -1234,8 +1251,6 @@ int run_graph(c2h_ctx* c, bool step, int pos) {
   }
   return C2H_OK;
 }
-
-thread_local std::string g_create_err;
 
 // `scratch`'s address on each device, looked up once per device (with that
 // device current) by the first c2h_create on it.
@@ -1342,6 +1357,7 @@ int c2h_create(const c2h_model_desc* desc, int device, c2h_ctx** out) {
   c->tok_host[0] = 0;
   c->tok_host[1] = -1;
   c->tok_host[2] = 0;
+  c->tok_host[3] = 0;
   int rc;
   if ((rc = noalloc_setup(c))) return bail(rc);
   if ((rc = dalloc(c, &c->state_dev, sizeof(C2hState)))) return bail(rc);
@@ -1519,6 +1535,7 @@ void c2h_destroy(c2h_ctx* c) {
   for (void* p : c->allocs) (void)hipFree(p);
   if (c->ids_dev) (void)hipFree(c->ids_dev);
   if (c->ids_y) (void)hipFree(c->ids_y);
+  if (c->paged_ws) (void)hipFree(c->paged_ws);
   if (c->state_ring) (void)hipHostFree(c->state_ring);
   if (c->stream) (void)hipStreamDestroy(c->stream);
   delete c;
@@ -2440,7 +2457,8 @@ int c2h_sync(c2h_ctx* c) {
   if (!c) return C2H_ERR_INVALID;
   HIPCHK(c, hipSetDevice(c->device));
   HIPCHK(c, hipStreamSynchronize(c->stream));
-  return check_wait_flag(c);
+  const int rc = check_wait_flag(c);
+  return rc ? rc : check_paged_flag(c);
 }
 
 int c2h_quantize_q8k(c2h_ctx* c, const float* x, int32_t cols, void* q8k_out) {
@@ -2532,6 +2550,350 @@ int c2h_gemv(c2h_ctx* c, int32_t type, const void* w, const void* xq, int32_t ro
     rc = fail(c, C2H_ERR_HIP, "copy out failed");
   cleanup();
   return rc;
+}
+
+// ---- operators for many sessions: descriptions checked on the host, then
+// one launch (or two) on the context's stream
+
+namespace {
+
+bool act_type(int t) { return t == C2H_F32 || t == C2H_F16 || t == C2H_BF16; }
+constexpr int64_t kMaxStride = (int64_t)1 << 40;  // elements: offsets stay far inside 64 bits
+
+// Whether vectors of `dim` elements at the given (stride, count) pairs lie
+// apart: each stride spans everything the smaller ones reach.
+bool apart(std::initializer_list<std::pair<int64_t, int64_t>> dims, int64_t dim) {
+  std::pair<int64_t, int64_t> d[3];
+  int n = 0;
+  for (const auto& x : dims)
+    if (x.second > 1) d[n++] = x;
+  std::sort(d, d + n);
+  int64_t reach = dim;
+  for (int i = 0; i < n; ++i) {
+    if (d[i].first < reach) return false;
+    reach = d[i].first * (d[i].second - 1) + reach;
+  }
+  return true;
+}
+
+int check_heads(c2h_ctx* c, const char* what, const c2h_heads* h, int type, int n_tokens, int n_heads, int head_dim,
+                bool written) {
+  const int es = type_bytes(type);
+  if (n_tokens == 0) return C2H_OK;  // an empty tensor may have no memory
+  if (!h || !h->data) return fail(c, C2H_ERR_INVALID, "%s: no data", what);
+  if (h->token_stride < 0 || h->head_stride < 0 || h->token_stride > kMaxStride || h->head_stride > kMaxStride)
+    return fail(c, C2H_ERR_INVALID, "%s: strides from 0 to 2^40 elements", what);
+  if ((reinterpret_cast<uintptr_t>(h->data) | (uintptr_t)(h->token_stride * es) | (uintptr_t)(h->head_stride * es)) & 15)
+    return fail(c, C2H_ERR_INVALID, "%s: data and strides must be multiples of 16 bytes", what);
+  if (written && !apart({{h->token_stride, n_tokens}, {h->head_stride, n_heads}}, head_dim))
+    return fail(c, C2H_ERR_INVALID, "%s: vectors overlap", what);
+  return C2H_OK;
+}
+
+HeadRows head_rows(const c2h_heads* h, int type) {
+  if (!h) return HeadRows{nullptr, 0, 0};
+  return HeadRows{reinterpret_cast<char*>(h->data), h->token_stride * type_bytes(type), h->head_stride * type_bytes(type)};
+}
+
+int check_paged(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b) {
+  if (!kv || !b) return fail(c, C2H_ERR_INVALID, "no cache or batch description");
+  if (!act_type(kv->type) && kv->type != C2H_F8_E4M3) return fail(c, C2H_ERR_UNSUPPORTED, "cache type %d", kv->type);
+  if (kv->page_size < PAGED_MIN_PAGE || kv->page_size > PAGED_MAX_PAGE || (kv->page_size & (kv->page_size - 1)))
+    return fail(c, C2H_ERR_UNSUPPORTED, "page_size %d: a power of two from %d to %d", kv->page_size, PAGED_MIN_PAGE,
+                PAGED_MAX_PAGE);
+  if (kv->head_dim < 16 || kv->head_dim > 256 || kv->head_dim % 16)
+    return fail(c, C2H_ERR_UNSUPPORTED, "head_dim %d: a multiple of 16 up to 256", kv->head_dim);
+  if (kv->n_pages < 1 || kv->n_kv_heads < 1 || kv->n_kv_heads > 1024)
+    return fail(c, C2H_ERR_INVALID, "a pool has pages, and 1 to 1024 KV heads");
+  const int es = type_bytes(kv->type);
+  if (!kv->k || !kv->v || kv->k == kv->v) return fail(c, C2H_ERR_INVALID, "keys and values need memory of their own");
+  const int64_t st[3] = {kv->page_stride, kv->token_stride, kv->head_stride};
+  uintptr_t low = reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v);
+  for (int64_t x : st) {
+    if (x < 0 || x > kMaxStride / 1024) return fail(c, C2H_ERR_INVALID, "cache strides from 0 to 2^30 elements");
+    low |= (uintptr_t)(x * es);
+  }
+  if (low & 15) return fail(c, C2H_ERR_INVALID, "cache pointers and strides must be multiples of 16 bytes");
+  if (!apart({{st[0], kv->n_pages}, {st[1], kv->page_size}, {st[2], kv->n_kv_heads}}, kv->head_dim))
+    return fail(c, C2H_ERR_INVALID, "cache vectors overlap");
+  if (b->n_seqs < 0 || b->n_seqs > (1 << 20)) return fail(c, C2H_ERR_INVALID, "%d sessions", b->n_seqs);
+  if (b->max_len < 0 || b->max_len > (1 << 30)) return fail(c, C2H_ERR_INVALID, "max_len %d", b->max_len);
+  if (b->n_seqs > 0 && (!b->block_table || !b->seq_lens)) return fail(c, C2H_ERR_INVALID, "no block table or lengths");
+  if (b->table_stride < 0 || b->table_stride > kMaxStride ||
+      b->table_stride < ((int64_t)b->max_len + kv->page_size - 1) / kv->page_size)
+    return fail(c, C2H_ERR_INVALID, "a table row of %lld pages of %d tokens does not cover max_len %d",
+                (long long)b->table_stride, kv->page_size, b->max_len);
+  return C2H_OK;
+}
+
+PagedKV paged_kv(const c2h_paged_kv* kv) {
+  const int es = type_bytes(kv->type);
+  PagedKV r;
+  r.k = reinterpret_cast<char*>(kv->k);
+  r.v = reinterpret_cast<char*>(kv->v);
+  r.page_stride = kv->page_stride * es;
+  r.token_stride = kv->token_stride * es;
+  r.head_stride = kv->head_stride * es;
+  r.k_scale = kv->k_scale;
+  r.v_scale = kv->v_scale;
+  r.n_pages = kv->n_pages;
+  r.page_shift = __builtin_ctz(kv->page_size);
+  r.n_kv_heads = kv->n_kv_heads;
+  r.head_dim = kv->head_dim;
+  return r;
+}
+
+PagedBatch paged_batch(const c2h_paged_batch* b) {
+  return PagedBatch{b->block_table, b->table_stride, b->seq_lens, b->n_seqs, b->max_len};
+}
+
+int check_rope(c2h_ctx* c, const c2h_rope* r, int head_dim) {
+  if (r->rot_dim < 8 || r->rot_dim > C2H_ROPE_MAX_DIM || r->rot_dim % 8 ||
+      (r->layout != C2H_ROPE_HALF && r->layout != C2H_ROPE_INTERLEAVED))
+    return fail(c, C2H_ERR_INVALID, "a rotation that c2h_rope_init did not fill");
+  if (r->rot_dim > head_dim) return fail(c, C2H_ERR_INVALID, "rot_dim %d exceeds head_dim %d", r->rot_dim, head_dim);
+  return C2H_OK;
+}
+
+RopeTab rope_tab(const c2h_rope* r) {
+  RopeTab t;
+  memset(&t, 0, sizeof(t));
+  t.mscale = 1.0f;
+  if (!r) return t;  // rot_dim 0: everything is copied
+  static_assert(sizeof(t.turns) == sizeof(r->turns), "one frequency per pair");
+  t.rot_dim = r->rot_dim;
+  t.layout = r->layout;
+  t.mscale = r->mscale;
+  memcpy(t.turns, r->turns, sizeof(t.turns));
+  return t;
+}
+
+// The launch's shape: workgroups per row, and the workspace their parts meet in.
+int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int n_heads, int window, PagedAttnParams* P,
+              size_t* bytes) {
+  if (n_heads < 1 || n_heads > 65536 || n_heads % kv->n_kv_heads)
+    return fail(c, C2H_ERR_INVALID, "%d query heads over %d KV heads", n_heads, kv->n_kv_heads);
+  if (window < 0) return fail(c, C2H_ERR_INVALID, "window %d", window);
+  P->n_heads = n_heads;
+  P->group = n_heads / kv->n_kv_heads;
+  P->n_tiles = (P->group + ATTN_HEADS - 1) / ATTN_HEADS;
+  P->window = window;
+  const int span = window > 0 ? std::min(window, b->max_len) : b->max_len;
+  P->chunk = attn_chunk((int64_t)b->n_seqs * kv->n_kv_heads * P->n_tiles, span);
+  P->n_chunks = std::max(1, chunks_of(Span{0, span}, P->chunk));
+  const int64_t parts = (int64_t)b->n_seqs * n_heads * P->n_chunks;
+  if (parts > 0x7fffffff) return fail(c, C2H_ERR_UNSUPPORTED, "%lld parts of rows exceed one launch", (long long)parts);
+  *bytes = P->n_chunks > 1 ? (size_t)parts * (kv->head_dim + 2) * 4 : 0;
+  return C2H_OK;
+}
+
+}  // namespace
+
+int c2h_rope_init(const c2h_rope_desc* d, c2h_rope* r) {
+  if (!d || !r) return fail(nullptr, C2H_ERR_INVALID, "no description or result");
+  if (d->rot_dim < 8 || d->rot_dim > C2H_ROPE_MAX_DIM || d->rot_dim % 8)
+    return fail(nullptr, C2H_ERR_UNSUPPORTED, "rot_dim %d: a multiple of 8 up to %d", d->rot_dim, C2H_ROPE_MAX_DIM);
+  if (d->layout != C2H_ROPE_HALF && d->layout != C2H_ROPE_INTERLEAVED)
+    return fail(nullptr, C2H_ERR_INVALID, "layout %d", d->layout);
+  if (!(d->base > 1.0) || !std::isfinite(d->base) || !std::isfinite(d->mscale) || !(d->factor >= 1.0) ||
+      !std::isfinite(d->factor) || d->orig_ctx < 0)
+    return fail(nullptr, C2H_ERR_INVALID, "base above 1, factor from 1, finite mscale, orig_ctx from 0");
+  const bool yarn = d->orig_ctx > 0 && d->factor > 1.0;
+  if (yarn && (!(d->beta_fast > 0.0) || !(d->beta_slow > 0.0) || !std::isfinite(d->beta_fast) || !std::isfinite(d->beta_slow)))
+    return fail(nullptr, C2H_ERR_INVALID, "beta_fast and beta_slow are positive");
+  const int n = d->rot_dim / 2;
+  for (int i = 0; d->freq_factors && i < n; ++i)
+    if (!(d->freq_factors[i] > 0.0f) || !std::isfinite(d->freq_factors[i]))
+      return fail(nullptr, C2H_ERR_INVALID, "freq_factors are positive");
+  const double pi = 3.14159265358979323846;
+  auto corner = [&](double t) { return d->rot_dim * std::log(d->orig_ctx / (2.0 * pi * t)) / (2.0 * std::log(d->base)); };
+  const double lo = yarn ? std::max(std::floor(corner(d->beta_fast)), 0.0) : 0.0;
+  const double hi = yarn ? std::min(std::ceil(corner(d->beta_slow)), d->rot_dim - 1.0) : 0.0;
+  memset(r, 0, sizeof(*r));
+  r->rot_dim = d->rot_dim;
+  r->layout = d->layout;
+  r->mscale = (float)d->mscale;
+  for (int i = 0; i < n; ++i) {
+    double f = std::pow(d->base, -2.0 * i / d->rot_dim);
+    if (d->freq_factors) f /= (double)d->freq_factors[i];
+    if (yarn) {
+      const double ramp = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.0), 1.0);
+      f = f * (1.0 - ramp) + f / d->factor * ramp;
+    } else {
+      f /= d->factor;
+    }
+    r->turns[i] = f / (2.0 * pi);
+  }
+  return C2H_OK;
+}
+
+int c2h_rope_dev(c2h_ctx* c, const c2h_rope* rope, int32_t type, const c2h_heads* x, const int32_t* positions,
+                 int32_t n_tokens, int32_t n_heads, int32_t head_dim, const c2h_heads* y) {
+  if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
+  if (n_tokens < 0 || n_heads < 1 || n_heads > 65536) return fail(c, C2H_ERR_INVALID, "%d tokens of %d heads", n_tokens, n_heads);
+  if (head_dim < 8 || head_dim > C2H_ROPE_MAX_DIM || head_dim % 8)
+    return fail(c, C2H_ERR_UNSUPPORTED, "head_dim %d: a multiple of 8 up to %d", head_dim, C2H_ROPE_MAX_DIM);
+  if (!rope || (n_tokens > 0 && !positions)) return fail(c, C2H_ERR_INVALID, "no rotation or positions");
+  int rc;
+  if ((rc = check_rope(c, rope, head_dim)) || (rc = check_heads(c, "x", x, type, n_tokens, n_heads, head_dim, false)) ||
+      (rc = check_heads(c, "y", y, type, n_tokens, n_heads, head_dim, true)))
+    return rc;
+  if (!c) return fail(c, C2H_ERR_INVALID, "no context");
+  if (n_tokens == 0) return C2H_OK;
+  HIPCHK(c, hipSetDevice(c->device));
+  RopeParams P;
+  memset(&P, 0, sizeof(P));
+  P.q = head_rows(x, type);
+  P.qo = head_rows(y, type);
+  P.positions = positions;
+  P.n_tokens = n_tokens;
+  P.n_q = n_heads;
+  P.head_dim = head_dim;
+  P.rope = rope_tab(rope);
+  launch_rope(P, type, type, false, c->stream);
+  HIPCHK(c, hipGetLastError());
+  return C2H_OK;
+}
+
+int c2h_paged_append_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, const int32_t* token_start,
+                         int32_t n_tokens, const c2h_rope* rope, int32_t type, const c2h_heads* k, const c2h_heads* v,
+                         int32_t n_heads, const c2h_heads* q, const c2h_heads* q_out) {
+  int rc = check_paged(c, kv, b);
+  if (rc) return rc;
+  if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
+  if (n_tokens < 0 || (!token_start && n_tokens != b->n_seqs))
+    return fail(c, C2H_ERR_INVALID, "%d tokens for %d sessions without token_start", n_tokens, b->n_seqs);
+  if (rope && (rc = check_rope(c, rope, kv->head_dim))) return rc;
+  if ((rc = check_heads(c, "k", k, type, n_tokens, kv->n_kv_heads, kv->head_dim, false)) ||
+      (rc = check_heads(c, "v", v, type, n_tokens, kv->n_kv_heads, kv->head_dim, false)))
+    return rc;
+  if (q || q_out) {
+    if (n_heads < 1 || n_heads > 65536) return fail(c, C2H_ERR_INVALID, "%d query heads", n_heads);
+    if ((rc = check_heads(c, "q", q, type, n_tokens, n_heads, kv->head_dim, false)) ||
+        (rc = check_heads(c, "q_out", q_out, type, n_tokens, n_heads, kv->head_dim, true)))
+      return rc;
+  }
+  if (!c) return fail(c, C2H_ERR_INVALID, "no context");
+  if (n_tokens == 0 || b->n_seqs == 0) return C2H_OK;
+  HIPCHK(c, hipSetDevice(c->device));
+  RopeParams P;
+  memset(&P, 0, sizeof(P));
+  P.q = head_rows(q, type);
+  P.qo = head_rows(q_out, type);
+  P.k = head_rows(k, type);
+  P.v = head_rows(v, type);
+  P.kv = paged_kv(kv);
+  P.b = paged_batch(b);
+  P.token_start = token_start;
+  P.n_tokens = n_tokens;
+  P.n_q = q ? n_heads : 0;
+  P.n_kv = kv->n_kv_heads;
+  P.head_dim = kv->head_dim;
+  P.err = c->tok_host + 3;
+  P.rope = rope_tab(rope);
+  launch_rope(P, type, kv->type, true, c->stream);
+  HIPCHK(c, hipGetLastError());
+  return C2H_OK;
+}
+
+int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* b, int32_t n_heads, int32_t window,
+                             size_t* bytes) {
+  if (!bytes) return fail(nullptr, C2H_ERR_INVALID, "no result");
+  *bytes = 0;
+  const int rc = check_paged(nullptr, kv, b);
+  if (rc) return rc;
+  PagedAttnParams P;
+  return plan_attn(nullptr, kv, b, n_heads, window, &P, bytes);
+}
+
+int c2h_paged_attn_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int32_t type, int32_t n_heads,
+                       float scale, int32_t window, const c2h_heads* q, const c2h_heads* out) {
+  int rc = check_paged(c, kv, b);
+  if (rc) return rc;
+  if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
+  PagedAttnParams P;
+  memset(&P, 0, sizeof(P));
+  size_t bytes = 0;
+  if ((rc = plan_attn(c, kv, b, n_heads, window, &P, &bytes)) ||
+      (rc = check_heads(c, "q", q, type, b->n_seqs, n_heads, kv->head_dim, false)) ||
+      (rc = check_heads(c, "out", out, type, b->n_seqs, n_heads, kv->head_dim, true)))
+    return rc;
+  if (!std::isfinite(scale)) return fail(c, C2H_ERR_INVALID, "scale is not finite");
+  if (!c) return fail(c, C2H_ERR_INVALID, "no context");
+  if (b->n_seqs == 0) return C2H_OK;
+  HIPCHK(c, hipSetDevice(c->device));
+  if (bytes > c->paged_ws_bytes) {
+    HIPCHK(c, hipStreamSynchronize(c->stream));
+    if (c->paged_ws) (void)hipFree(c->paged_ws);
+    c->paged_ws = nullptr;
+    c->paged_ws_bytes = 0;
+    void* p = nullptr;
+    HIPCHK(c, hipMalloc(&p, bytes));
+    c->paged_ws = reinterpret_cast<float*>(p);
+    c->paged_ws_bytes = bytes;
+  }
+  P.kv = paged_kv(kv);
+  P.b = paged_batch(b);
+  P.q = head_rows(q, type);
+  P.out = head_rows(out, type);
+  P.type = type;
+  P.scale_log2 = (float)((double)scale * 1.44269504088896340736);
+  P.part_o = c->paged_ws;
+  P.part_ml = c->paged_ws ? c->paged_ws + (size_t)b->n_seqs * n_heads * P.n_chunks * kv->head_dim : nullptr;
+  P.err = c->tok_host + 3;
+  launch_paged_attn(P, kv->type, c->stream);
+  HIPCHK(c, hipGetLastError());
+  return C2H_OK;
+}
+
+int c2h_rmsnorm_q8k_dev(c2h_ctx* c, int32_t type, const void* x, int64_t x_stride, const void* residual,
+                        int64_t residual_stride, const float* w, float eps, int32_t n_rows, int32_t cols, void* sum_out,
+                        int64_t sum_stride, void* q8k_out, float* y_out, int64_t y_stride) {
+  if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
+  if (n_rows < 0) return fail(c, C2H_ERR_INVALID, "%d rows", n_rows);
+  if (cols < 256 || cols > 16384 || cols % 8)
+    return fail(c, C2H_ERR_UNSUPPORTED, "%d columns: a multiple of 8 from 256 to 16384", cols);
+  if (n_rows > 0 && (!x || !w || !q8k_out || (residual != nullptr) != (sum_out != nullptr)))
+    return fail(c, C2H_ERR_INVALID, "x, w and q8k_out are required, residual and sum_out come together");
+  if (!(eps >= 0.0f)) return fail(c, C2H_ERR_INVALID, "eps from 0");
+  const int es = type_bytes(type);
+  uintptr_t low = reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(y_out);
+  const struct {
+    const void* p;
+    int64_t stride;
+    int es;
+    bool written;
+  } rows[4] = {{x, x_stride, es, false}, {residual, residual_stride, es, false}, {sum_out, sum_stride, es, true},
+               {y_out, y_stride, 4, true}};
+  for (const auto& r : rows) {
+    if (!r.p) continue;
+    if (r.stride < 0 || r.stride > kMaxStride || (r.written && n_rows > 1 && r.stride < cols))
+      return fail(c, C2H_ERR_INVALID, "a row stride of %lld elements for %d columns", (long long)r.stride, cols);
+    low |= reinterpret_cast<uintptr_t>(r.p) | (uintptr_t)(r.stride * r.es);
+  }
+  if ((low & 15) || (reinterpret_cast<uintptr_t>(q8k_out) & 3))
+    return fail(c, C2H_ERR_INVALID, "rows and w must be multiples of 16 bytes, q8k_out of 4");
+  if (!c) return fail(c, C2H_ERR_INVALID, "no context");
+  if (n_rows == 0) return C2H_OK;
+  HIPCHK(c, hipSetDevice(c->device));
+  NormQ8Params P;
+  memset(&P, 0, sizeof(P));
+  P.x = reinterpret_cast<const char*>(x);
+  P.r = reinterpret_cast<const char*>(residual);
+  P.sum = reinterpret_cast<char*>(sum_out);
+  P.x_stride = x_stride * es;
+  P.r_stride = residual_stride * es;
+  P.sum_stride = sum_stride * es;
+  P.w = w;
+  P.y = y_out;
+  P.y_stride = y_stride;
+  P.q8k = reinterpret_cast<uint8_t*>(q8k_out);
+  P.eps = eps;
+  P.n_rows = n_rows;
+  P.cols = cols;
+  launch_norm_q8(P, type, c->stream);
+  HIPCHK(c, hipGetLastError());
+  return C2H_OK;
 }
 
 int c2h_copy_bench(c2h_ctx* c, int64_t bytes, int32_t reps, float* ms) {

@@ -27,6 +27,7 @@
 // loads the next phase needs while the rest stay in flight.
 #include "c2h_device.h"
 #include "c2h_kernels.h"
+#include "c2h_paged.h"
 
 namespace c2h {
 
@@ -497,6 +498,136 @@ __device__ __forceinline__ float rms_scale(float v) {
     return (float)__builtin_fma(y, r, y);
   }
   return (float)(1.0 / sqrt((double)v));
+}
+
+// ---------------------------------- RMSNorm of a batch of rows to Q8_K rows
+
+// The 292-byte Q8_K blocks in memory as quantize_blocks addresses its row:
+// block b's f32 d, 256 int8 quants and 16 int16 sums, 73 dwords in all.
+struct Q8KOut {
+  uint32_t (*q)[73];
+  int16_t (*bs)[146];
+  struct Scale {
+    float* p;
+    __device__ float& operator[](int b) const { return p[b * 73]; }
+  } d;
+  __device__ explicit Q8KOut(uint8_t* y)
+      : q(reinterpret_cast<uint32_t(*)[73]>(y + 4)), bs(reinterpret_cast<int16_t(*)[146]>(y + 260)),
+        d{reinterpret_cast<float*>(y)} {}
+};
+
+// Elements 4i .. 4i+3 of a row.
+template <int T>
+__device__ __forceinline__ float4 load_row4(const char* row, int i) {
+  if constexpr (T == PT_F32) {
+    return reinterpret_cast<const float4*>(row)[i];
+  } else {
+    const uint2 u = reinterpret_cast<const uint2*>(row)[i];
+    if constexpr (T == PT_BF16)
+      return make_float4(bits_f32(u.x << 16), bits_f32(u.x & 0xffff0000u), bits_f32(u.y << 16), bits_f32(u.y & 0xffff0000u));
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    const h4 h = __builtin_bit_cast(h4, u);
+    return make_float4((float)h.x, (float)h.y, (float)h.z, (float)h.w);
+  }
+}
+// Stores v rounded to the type and returns what was stored.
+template <int T>
+__device__ __forceinline__ float4 store_row4(char* row, int i, float4 v) {
+  if constexpr (T == PT_F32) {
+    reinterpret_cast<float4*>(row)[i] = v;
+    return v;
+  } else if constexpr (T == PT_F16) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    const h4 h = {(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
+    reinterpret_cast<uint2*>(row)[i] = __builtin_bit_cast(uint2, h);
+    return make_float4((float)h.x, (float)h.y, (float)h.z, (float)h.w);
+  } else {
+    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+    const b4 b = {(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
+    reinterpret_cast<uint2*>(row)[i] = __builtin_bit_cast(uint2, b);
+    return make_float4((float)b.x, (float)b.y, (float)b.z, (float)b.w);
+  }
+}
+
+// A workgroup per row: wave w of NW holds the 256-element blocks w, w + NW,
+// ... (BPW of them), lane l elements 4l .. 4l+3 of each, as quantize_blocks
+// takes them; the row is read once and stays in registers.  The squares are
+// summed in 64 bits, so that the order of the sum does not reach the quants.
+template <int T, int BPW, int NW>
+__global__ void __launch_bounds__(64 * NW) k_norm_q8(NormQ8Params P) {
+  __shared__ double part[NW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const char* x = P.x + row * P.x_stride;
+  float4 v[BPW];
+#pragma unroll
+  for (int i = 0; i < BPW; ++i) {
+    const int c4 = (wave + NW * i) * 64 + lane;
+    v[i] = 4 * c4 < P.cols ? load_row4<T>(x, c4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  if (P.r) {
+    const char* r = P.r + row * P.r_stride;
+    char* sum = P.sum + row * P.sum_stride;
+#pragma unroll
+    for (int i = 0; i < BPW; ++i) {
+      const int c4 = (wave + NW * i) * 64 + lane;
+      if (4 * c4 < P.cols) {
+        const float4 a = load_row4<T>(r, c4);
+        v[i] = store_row4<T>(sum, c4, make_float4(v[i].x + a.x, v[i].y + a.y, v[i].z + a.z, v[i].w + a.w));
+      }
+    }
+  }
+  double ss = 0.0;
+#pragma unroll
+  for (int i = 0; i < BPW; ++i)
+    ss += ((double)v[i].x * v[i].x + (double)v[i].y * v[i].y) + ((double)v[i].z * v[i].z + (double)v[i].w * v[i].w);
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) ss += __shfl_xor(ss, m);
+  if (lane == 0) part[wave] = ss;
+  __syncthreads();
+  ss = 0.0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) ss += part[i];
+  const float scale = (float)(1.0 / sqrt(ss / (double)P.cols + (double)P.eps));
+#pragma unroll
+  for (int i = 0; i < BPW; ++i) {
+    const int c4 = (wave + NW * i) * 64 + lane;
+    if (4 * c4 < P.cols) {
+      const float4 w = reinterpret_cast<const float4*>(P.w)[c4];
+      v[i] = make_float4((v[i].x * scale) * w.x, (v[i].y * scale) * w.y, (v[i].z * scale) * w.z, (v[i].w * scale) * w.w);
+      if (P.y) reinterpret_cast<float4*>(P.y + row * P.y_stride)[c4] = v[i];
+    }
+  }
+  const int nb = P.cols / QK_K;
+  Q8KOut out(P.q8k + row * nb * BS_Q8K);
+  quantize_blocks<BPW>(v, wave, NW, nb, out);
+}
+
+namespace {
+template <int T>
+void launch_norm_q8_t(const NormQ8Params& P, hipStream_t st) {
+  const int nbt = (P.cols + QK_K - 1) / QK_K;
+  const dim3 grid(P.n_rows);
+  if (nbt <= 4)
+    hipLaunchKernelGGL((k_norm_q8<T, 1, 4>), grid, dim3(256), 0, st, P);
+  else if (nbt <= 8)
+    hipLaunchKernelGGL((k_norm_q8<T, 2, 4>), grid, dim3(256), 0, st, P);
+  else if (nbt <= 16)
+    hipLaunchKernelGGL((k_norm_q8<T, 4, 4>), grid, dim3(256), 0, st, P);
+  else if (nbt <= 32)
+    hipLaunchKernelGGL((k_norm_q8<T, 4, 8>), grid, dim3(512), 0, st, P);
+  else
+    hipLaunchKernelGGL((k_norm_q8<T, 4, 16>), grid, dim3(1024), 0, st, P);
+}
+}  // namespace
+
+void launch_norm_q8(const NormQ8Params& P, int type, hipStream_t st) {
+  if (type == PT_F32)
+    launch_norm_q8_t<PT_F32>(P, st);
+  else if (type == PT_F16)
+    launch_norm_q8_t<PT_F16>(P, st);
+  else
+    launch_norm_q8_t<PT_BF16>(P, st);
 }
 
 // rms_scale against the IEEE operations over the bit patterns [lo, lo + n);

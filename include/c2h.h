@@ -8,6 +8,11 @@
  * (engine/pool.go:22-42 keeps unsynchronised task state).
  *
  * Status: 0 = OK, < 0 = error; c2h_last_error() describes the last failure.
+ *
+ * Operators with a _dev suffix take device pointers of the context's GPU,
+ * run on the context's stream and return without synchronising: what they
+ * read must be complete before the call (another stream's work waited for),
+ * and what they wrote may be used elsewhere after c2h_sync.
  */
 #ifndef C2H_H
 #define C2H_H
@@ -32,6 +37,13 @@ extern "C" {
 #define C2H_Q8_0 8
 #define C2H_Q4_K 12
 #define C2H_Q6_K 14
+/* Element types of the operators over many sessions (ggml's numbers; e4m3,
+ * which ggml has none for, is this library's): activations are F32, F16 or
+ * BF16, a paged cache also holds 8-bit floats (OCP e4m3: no infinities,
+ * largest 448). */
+#define C2H_F16 1
+#define C2H_BF16 30
+#define C2H_F8_E4M3 100
 
 /* Tensor roles: what engine/model.go:114-207 binds.  Per-layer roles take
  * the layer index; global roles ignore it. */
@@ -247,6 +259,179 @@ int c2h_logits_ids(c2h_ctx* ctx, const int32_t* ids, int32_t n_ids, float* logit
 /* Device-pointer form (ids and logits in device memory, logits n_vocab
  * floats); runs on the context stream without synchronising. */
 int c2h_logits_ids_dev(c2h_ctx* ctx, const int32_t* ids, int32_t n_ids, float* logits);
+
+/* ---- operators for many sessions ------------------------------------------ */
+
+/* No counterpart in the reference, which serves one session at a time from a
+ * contiguous cache.  These operators are one decode layer's work on a batch
+ * of sessions that share a pool of pages: c2h_rmsnorm_q8k_dev feeds the
+ * projections (c2h_gemv_dev per row), c2h_paged_append_dev rotates and
+ * stores what they return, c2h_paged_attn_dev attends.  They work on any
+ * context (desc == NULL included).  A context's calls run one after another
+ * on its stream; calls on several contexts may run at once as long as none
+ * writes what another reads. */
+
+/* Head vectors of a run of tokens, in device memory: element d of head h of
+ * token t is data[t * token_stride + h * head_stride + d], strides in
+ * elements, so the parts of a fused projection's rows are described as they
+ * lie.  data and both strides are multiples of 16 bytes and no stride is
+ * negative; vectors that are written do not overlap. */
+typedef struct c2h_heads {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} c2h_heads;
+
+/* Rotary positions.  Pair i of a head (i < rot_dim / 2) is turned by
+ * pos * f_i, f_i = base^(-2 i / rot_dim), and multiplied by mscale:
+ *   u' = mscale (u cos - v sin),  v' = mscale (u sin + v cos),
+ * with (u, v) = (x[i], x[i + rot_dim / 2]) in the half layout (the
+ * reference's, tensor/ops.go:228-286) and (x[2i], x[2i + 1]) in the
+ * interleaved one.  Elements from rot_dim on are copied.  For contexts
+ * longer than the trained one the frequencies are scaled:
+ *   freq_factors != NULL         f_i / freq_factors[i]
+ *   factor > 1, orig_ctx == 0    f_i / factor (linear)
+ *   factor > 1, orig_ctx > 0     YaRN: f_i (1 - r_i) + (f_i / factor) r_i,
+ *                                r_i = clamp((i - lo) / max(hi - lo, 0.001), 0, 1),
+ *                                lo, hi = max(floor(c(beta_fast)), 0),
+ *                                min(ceil(c(beta_slow)), rot_dim - 1),
+ *                                c(t) = rot_dim ln(orig_ctx / (2 pi t)) / (2 ln base)
+ * (factors first, then the other).  YaRN's attention factor is the caller's
+ * mscale.  Angles are formed in 64 bits, so positions keep their accuracy
+ * however far; a negative position turns back. */
+#define C2H_ROPE_HALF 0
+#define C2H_ROPE_INTERLEAVED 1
+#define C2H_ROPE_MAX_DIM 256
+typedef struct c2h_rope_desc {
+  int32_t rot_dim; /* 8 .. C2H_ROPE_MAX_DIM, a multiple of 8 */
+  int32_t layout;  /* C2H_ROPE_* */
+  double base;
+  double mscale;   /* 1 for none */
+  double factor;   /* 1 for none */
+  int32_t orig_ctx;
+  int32_t reserved;
+  double beta_fast, beta_slow;
+  const float* freq_factors; /* host, rot_dim / 2 floats, or NULL; read during c2h_rope_init only */
+} c2h_rope_desc;
+
+/* A rotation ready for use: plain data that c2h_rope_init fills on the host
+ * (no GPU, no context), to be kept and copied as the caller likes. */
+typedef struct c2h_rope {
+  int32_t rot_dim;
+  int32_t layout;
+  float mscale;
+  int32_t reserved;
+  double turns[C2H_ROPE_MAX_DIM / 2]; /* f_i / (2 pi) */
+} c2h_rope;
+int c2h_rope_init(const c2h_rope_desc* desc, c2h_rope* rope);
+
+/* y = x rotated, for n_tokens tokens of n_heads heads of head_dim elements
+ * (a multiple of 8 up to 256, at least rot_dim) of type F32, F16 or BF16;
+ * token t stands at positions[t] (device, int32).  32-bit arithmetic, one
+ * rounding to the type.  y may be x itself (same pointer and strides);
+ * otherwise they must not overlap. */
+int c2h_rope_dev(c2h_ctx* ctx, const c2h_rope* rope, int32_t type, const c2h_heads* x, const int32_t* positions,
+                 int32_t n_tokens, int32_t n_heads, int32_t head_dim, const c2h_heads* y);
+
+/* A pool of pages of keys and values of one layer, in device memory.
+ * Element d of KV head h of the token in slot t of page p is
+ * k[p * page_stride + t * token_stride + h * head_stride + d] (v the same,
+ * its own pointer): either order of tokens and heads within a page, or a
+ * pool whose pages hold K and V side by side.  Strides are in elements; the
+ * pointers and strides are multiples of 16 bytes, and no two vectors
+ * overlap.  F8_E4M3 pools hold x / scale of the head, rounded to nearest
+ * even and saturated at +-448 (NaN stays NaN); k_scale and v_scale are
+ * n_kv_heads device floats each (NULL: 1). */
+typedef struct c2h_paged_kv {
+  void* k;
+  void* v;
+  int32_t type;       /* C2H_F32, C2H_F16, C2H_BF16 or C2H_F8_E4M3 */
+  int32_t n_pages;
+  int32_t page_size;  /* tokens: a power of two from 8 to 1024 */
+  int32_t n_kv_heads;
+  int32_t head_dim;   /* a multiple of 16 up to 256 */
+  int32_t reserved;
+  int64_t page_stride;
+  int64_t token_stride;
+  int64_t head_stride;
+  const float* k_scale;
+  const float* v_scale;
+} c2h_paged_kv;
+
+/* The sessions of a call: positions [j * page_size, (j+1) * page_size) of
+ * session s lie in page block_table[s * table_stride + j]; it holds
+ * seq_lens[s] positions, the call's own new ones included (0: no session in
+ * this row).  Table and lengths are device int32 and may change between
+ * calls; max_len is a bound of the lengths that the host knows (the launch
+ * is sized by it; table_stride * page_size covers it).
+ * The kernels check what they find there: a length below 0 or above
+ * max_len, or a page index outside [0, n_pages) where a position is held,
+ * reads and writes nothing outside the pool; such a session's attention
+ * rows are NaN, its appends are dropped, and the next c2h_sync returns
+ * C2H_ERR_RANGE. */
+typedef struct c2h_paged_batch {
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  int32_t n_seqs;
+  int32_t max_len;
+} c2h_paged_batch;
+
+/* Stores the keys and values of new tokens, and rotates the queries with
+ * them.  token_start (device, n_seqs + 1 ascending int32, the first 0) gives
+ * session s the tokens [token_start[s], token_start[s+1]), which are its
+ * last ones: the positions up to seq_lens[s] - 1.  NULL: one token per
+ * session, token s (n_tokens == n_seqs).  k and v are [n_tokens][n_kv_heads]
+ * vectors of `type` (F32, F16, BF16); K is stored rotated by `rope` (NULL:
+ * as it is), V as it is, each rounded once to the pool's type.  q (NULL:
+ * none), n_heads vectors per token, goes to q_out, rotated, in `type`;
+ * q_out may be q (same pointer and strides).  Tokens from
+ * token_start[n_seqs] on and those of sessions of length 0 are no tokens:
+ * their q_out rows are left as they were.  Pages shared between sessions
+ * are read only: no two tokens of a call may come to stand in one slot. */
+int c2h_paged_append_dev(c2h_ctx* ctx, const c2h_paged_kv* kv, const c2h_paged_batch* batch,
+                         const int32_t* token_start, int32_t n_tokens, const c2h_rope* rope, int32_t type,
+                         const c2h_heads* k, const c2h_heads* v, int32_t n_heads, const c2h_heads* q,
+                         const c2h_heads* q_out);
+
+/* Attention of one new token per session: for query head h of session s,
+ *   out = sum_j p_j v_j,  p = softmax_j(scale * q . k_j)
+ * over the positions j < seq_lens[s] (the last `window` of them where
+ * window > 0) of KV head h / (n_heads / n_kv_heads).  q and out are
+ * [n_seqs][n_heads] vectors of `type` (F32, F16, BF16), not overlapping.  A
+ * session of length 0 gets zeros.  Scores, softmax and sums are 32-bit, the
+ * result is rounded once to `type`; the same call on the same data gives the
+ * same bits (how long sessions are split follows from n_seqs, max_len,
+ * window and the pool's description alone).
+ * Work of several workgroups on one row meets in a workspace of the
+ * context, which c2h_paged_attn_workspace sizes; it grows, with a wait for
+ * the stream, in the first call that needs more than any before. */
+int c2h_paged_attn_dev(c2h_ctx* ctx, const c2h_paged_kv* kv, const c2h_paged_batch* batch, int32_t type,
+                       int32_t n_heads, float scale, int32_t window, const c2h_heads* q, const c2h_heads* out);
+
+/* Bytes of workspace that call takes, after the same checks of the
+ * descriptions (no GPU, no context; c2h_last_error(NULL) says what failed). */
+int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* batch, int32_t n_heads, int32_t window,
+                             size_t* bytes);
+
+/* RMSNorm with the residual's addition and Q8_K rows as its output: for each
+ * of n_rows rows of cols elements (256 .. 16384, a multiple of 8) of `type`
+ * (F32, F16, BF16)
+ *   s = x + residual (rounded to the type and stored to sum_out; s = x where
+ *       residual is NULL),
+ *   y = (s * f32(1 / sqrt(mean(s^2) + eps))) * w,
+ * the mean in 64 bits, the rest in 32, and y quantised as
+ * c2h_quantize_q8k_dev does: floor(cols / 256) blocks per row, the operand
+ * of c2h_gemv_dev, back to back in q8k_out (row r at r * (cols / 256) * 292
+ * bytes).  y_out (nullable) receives y as floats, all cols of it, for the
+ * formats whose products read f32 rows.  Rows of x, residual and sum_out are
+ * x_stride, residual_stride and sum_stride elements apart, those of y_out
+ * y_stride floats; pointers and strides are multiples of 16 bytes (q8k_out:
+ * 4).  sum_out is required with a residual (NULL without) and may be x or
+ * the residual itself (same pointer and stride). */
+int c2h_rmsnorm_q8k_dev(c2h_ctx* ctx, int32_t type, const void* x, int64_t x_stride, const void* residual,
+                        int64_t residual_stride, const float* w, float eps, int32_t n_rows, int32_t cols,
+                        void* sum_out, int64_t sum_stride, void* q8k_out, float* y_out, int64_t y_stride);
 
 /* ---- measurement --------------------------------------------------------- */
 

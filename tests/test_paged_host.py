@@ -1,0 +1,289 @@
+"""The operators over many sessions without a GPU: what their calls refuse
+(arguments are checked before the context is used), the frequencies that
+c2h_rope_init fills, and the index arithmetic of the kernels compiled as
+plain C++."""
+import ctypes as C
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from c2slm_amd import _lib as H
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+INVALID, UNSUPPORTED = -1, -3
+A = 0x10000  # an aligned address; nothing here reads or writes it
+
+
+def kv(**over):
+    d = dict(k=A, v=2 * A, type=H.BF16, n_pages=100, page_size=16, n_kv_heads=2, head_dim=64, reserved=0,
+             page_stride=16 * 128, token_stride=128, head_stride=64, k_scale=None, v_scale=None)
+    d.update(over)
+    return H.PagedKV(*[d[n] for n, _ in H.PagedKV._fields_])
+
+
+def batch(**over):
+    d = dict(block_table=A, table_stride=8, seq_lens=A, n_seqs=3, max_len=128)
+    d.update(over)
+    return H.PagedBatch(*[d[n] for n, _ in H.PagedBatch._fields_])
+
+
+def heads(data=A, token_stride=1024, head_stride=64):
+    return H.Heads(data, token_stride, head_stride)
+
+
+def refused(rc, code, word):
+    assert rc == code, (rc, H.lib().c2h_last_error(None))
+    assert word in H.lib().c2h_last_error(None).decode()
+
+
+BAD_CACHE = [
+    (dict(type=12), UNSUPPORTED, "type"), (dict(page_size=4), UNSUPPORTED, "page_size"),
+    (dict(page_size=24), UNSUPPORTED, "page_size"), (dict(page_size=2048), UNSUPPORTED, "page_size"),
+    (dict(head_dim=72), UNSUPPORTED, "head_dim"), (dict(head_dim=272), UNSUPPORTED, "head_dim"),
+    (dict(head_dim=0), UNSUPPORTED, "head_dim"), (dict(n_pages=0), INVALID, "pages"),
+    (dict(n_kv_heads=0), INVALID, "KV heads"), (dict(k=None), INVALID, "memory"), (dict(v=None), INVALID, "memory"),
+    (dict(v=A), INVALID, "memory of their own"), (dict(k=A + 8), INVALID, "16 bytes"),
+    (dict(token_stride=132), INVALID, "16 bytes"), (dict(token_stride=-128), INVALID, "strides"),
+    (dict(head_stride=32), INVALID, "overlap"), (dict(token_stride=64), INVALID, "overlap"),
+    (dict(page_stride=15 * 128), INVALID, "overlap"), (dict(page_stride=0), INVALID, "overlap"),
+    (dict(page_stride=1 << 50), INVALID, "strides"),
+]
+BAD_BATCH = [
+    (dict(n_seqs=-1), "sessions"), (dict(max_len=-1), "max_len"), (dict(max_len=(1 << 30) + 1), "max_len"),
+    (dict(block_table=None), "table"), (dict(seq_lens=None), "lengths"), (dict(max_len=129), "does not cover"),
+    (dict(table_stride=-1), "does not cover"),
+]
+
+
+@pytest.mark.parametrize("over,code,word", BAD_CACHE, ids=lambda v: str(v) if isinstance(v, dict) else "")
+def test_cache_descriptions_refused(over, code, word):
+    L, n, q = H.lib(), C.c_size_t(7), heads()
+    refused(L.c2h_paged_attn_workspace(kv(**over), batch(), 4, 0, C.byref(n)), code, word)
+    assert n.value == 0
+    refused(L.c2h_paged_attn_dev(None, kv(**over), batch(), H.F32, 4, 0.125, 0, q, q), code, word)
+    refused(L.c2h_paged_append_dev(None, kv(**over), batch(), None, 3, None, H.F32, q, q, 0, None, None), code, word)
+
+
+@pytest.mark.parametrize("over,word", BAD_BATCH, ids=lambda v: str(v) if isinstance(v, dict) else "")
+def test_batch_descriptions_refused(over, word):
+    L, n, q = H.lib(), C.c_size_t(7), heads()
+    refused(L.c2h_paged_attn_workspace(kv(), batch(**over), 4, 0, C.byref(n)), INVALID, word)
+    refused(L.c2h_paged_attn_dev(None, kv(), batch(**over), H.F32, 4, 0.125, 0, q, q), INVALID, word)
+    refused(L.c2h_paged_append_dev(None, kv(), batch(**over), None, 3, None, H.F32, q, q, 0, None, None), INVALID, word)
+
+
+def test_attention_arguments_refused():
+    L, q = H.lib(), heads()
+
+    def call(kv_=None, type=H.F32, n_heads=4, scale=0.125, window=0, q=q, out=q):
+        return L.c2h_paged_attn_dev(None, kv_ or kv(), batch(), type, n_heads, scale, window, q, out)
+
+    refused(call(type=H.F8_E4M3), UNSUPPORTED, "type")
+    refused(call(type=12), UNSUPPORTED, "type")
+    refused(call(n_heads=3), INVALID, "query heads")
+    refused(call(n_heads=0), INVALID, "query heads")
+    refused(call(window=-1), INVALID, "window")
+    refused(call(scale=float("nan")), INVALID, "scale")
+    refused(call(scale=float("inf")), INVALID, "scale")
+    refused(call(q=None), INVALID, "q: no data")
+    refused(call(q=heads(data=None)), INVALID, "q: no data")
+    refused(call(out=heads(data=A + 4)), INVALID, "out: data and strides")
+    refused(call(q=heads(token_stride=1026)), INVALID, "q: data and strides")
+    refused(call(q=heads(head_stride=-64)), INVALID, "q: strides")
+    refused(call(out=heads(token_stride=0)), INVALID, "out: vectors overlap")
+    refused(call(out=heads(head_stride=32)), INVALID, "out: vectors overlap")
+    refused(call(out=heads(token_stride=192)), INVALID, "out: vectors overlap")
+    refused(call(q=heads(token_stride=0)), INVALID, "no context")  # one query for all sessions is fine
+
+
+def test_append_and_rope_arguments_refused():
+    L, x, r = H.lib(), heads(), H.rope(64, 1e6)
+
+    def app(n=3, start=None, rope=None, type=H.F32, k=x, v=x, n_heads=0, q=None, q_out=None):
+        return L.c2h_paged_append_dev(None, kv(), batch(), start, n, rope, type, k, v, n_heads, q, q_out)
+
+    refused(app(n=4), INVALID, "4 tokens for 3 sessions")
+    refused(app(n=-1, start=A), INVALID, "tokens")
+    refused(app(type=H.F8_E4M3), UNSUPPORTED, "type")
+    refused(app(rope=H.Rope()), INVALID, "did not fill")
+    refused(app(rope=H.rope(128, 1e6)), INVALID, "rot_dim 128 exceeds head_dim 64")
+    refused(app(k=None), INVALID, "k: no data")
+    refused(app(v=heads(data=A + 2)), INVALID, "v: data")
+    refused(app(q=x, n_heads=4), INVALID, "q_out: no data")
+    refused(app(q_out=x, n_heads=4), INVALID, "q: no data")
+    refused(app(q=x, q_out=x), INVALID, "query heads")
+    refused(app(q=x, q_out=heads(token_stride=128), n_heads=4), INVALID, "q_out: vectors overlap")
+    refused(app(rope=r, q=x, q_out=x, n_heads=4), INVALID, "no context")
+    refused(app(n=9, start=A), INVALID, "no context")
+
+    def rope(rope=r, type=H.F32, x=x, pos=A, n=3, n_heads=4, hd=64, y=x):
+        return L.c2h_rope_dev(None, rope, type, x, pos, n, n_heads, hd, y)
+
+    refused(rope(rope=None), INVALID, "no rotation")
+    refused(rope(pos=None), INVALID, "positions")
+    refused(rope(type=H.F8_E4M3), UNSUPPORTED, "type")
+    refused(rope(n=-1), INVALID, "tokens")
+    refused(rope(n_heads=0), INVALID, "heads")
+    refused(rope(hd=60), UNSUPPORTED, "head_dim")
+    refused(rope(hd=264), UNSUPPORTED, "head_dim")
+    refused(rope(hd=56), INVALID, "exceeds")
+    refused(rope(y=heads(head_stride=32)), INVALID, "y: vectors overlap")
+    refused(rope(x=None), INVALID, "x: no data")
+    refused(rope(), INVALID, "no context")
+
+
+def test_norm_arguments_refused():
+    L = H.lib()
+
+    def norm(type=H.F32, x=A, xs=1024, r=None, rs=0, w=A, eps=1e-6, n=2, cols=896, s=None, ss=0, q=A, y=None, ys=0):
+        return L.c2h_rmsnorm_q8k_dev(None, type, x, xs, r, rs, w, eps, n, cols, s, ss, q, y, ys)
+
+    refused(norm(type=H.F8_E4M3), UNSUPPORTED, "type")
+    for cols in (248, 0, -256, 900, 16392):
+        refused(norm(cols=cols), UNSUPPORTED, "columns")
+    refused(norm(n=-1), INVALID, "rows")
+    refused(norm(x=None), INVALID, "required")
+    refused(norm(w=None), INVALID, "required")
+    refused(norm(q=None), INVALID, "required")
+    refused(norm(r=A, rs=1024), INVALID, "come together")
+    refused(norm(s=A, ss=1024), INVALID, "come together")
+    refused(norm(eps=-1.0), INVALID, "eps")
+    refused(norm(eps=float("nan")), INVALID, "eps")
+    refused(norm(x=A + 4), INVALID, "16 bytes")
+    refused(norm(xs=898), INVALID, "16 bytes")
+    refused(norm(q=A + 2), INVALID, "q8k_out of 4")
+    refused(norm(y=A, ys=512), INVALID, "row stride")
+    refused(norm(r=A, rs=1024, s=A, ss=0), INVALID, "row stride")
+    refused(norm(xs=-1024), INVALID, "row stride")
+    refused(norm(), INVALID, "no context")
+
+
+def test_workspace_follows_the_split():
+    # a batch that fills the GPU with whole sessions needs none; one long
+    # session is split, and its parts are head_dim + 2 floats per query head
+    assert H.paged_attn_workspace(kv(n_kv_heads=8, page_stride=16 * 512, token_stride=512),
+                                  batch(n_seqs=512, max_len=100), 16) == 0
+    one = batch(n_seqs=1, max_len=8192, table_stride=512)
+    got = H.paged_attn_workspace(kv(), one, 14)
+    assert got > 0 and got % (14 * (64 + 2) * 4) == 0
+    # a window bounds it
+    assert H.paged_attn_workspace(kv(), one, 14, window=100) == 0
+    assert H.paged_attn_workspace(kv(), batch(n_seqs=0), 14) == 0
+
+
+@pytest.mark.parametrize("over,code,word", [
+    (dict(rot_dim=4), UNSUPPORTED, "rot_dim"), (dict(rot_dim=60), UNSUPPORTED, "rot_dim"),
+    (dict(rot_dim=264), UNSUPPORTED, "rot_dim"), (dict(base=1.0), INVALID, "base"), (dict(base=float("inf")), INVALID, "base"),
+    (dict(base=float("nan")), INVALID, "base"), (dict(factor=0.5), INVALID, "factor"),
+    (dict(factor=float("nan")), INVALID, "factor"), (dict(mscale=float("inf")), INVALID, "mscale"),
+    (dict(orig_ctx=-1), INVALID, "orig_ctx"), (dict(factor=4.0, orig_ctx=4096, beta_fast=0.0), INVALID, "beta"),
+    (dict(freq_factors=np.zeros(32)), INVALID, "freq_factors"),
+], ids=lambda v: str(v) if isinstance(v, dict) else "")
+def test_rope_descriptions_refused(over, code, word):
+    args = dict(rot_dim=64, base=1e6)
+    args.update(over)
+    with pytest.raises(H.C2hError) as e:
+        H.rope(**args)
+    assert e.value.code == code and word in str(e.value)
+
+
+def test_rope_frequencies():
+    n = np.arange(32)
+    f = 1e6 ** (-n / 32.0)
+    got = lambda r: np.array(r.turns[:r.rot_dim // 2]) * 2 * math.pi  # noqa: E731
+    # a few roundings of 64 bits each
+    np.testing.assert_allclose(got(H.rope(64, 1e6)), f, rtol=2e-15)
+    np.testing.assert_allclose(got(H.rope(64, 1e6, factor=4.0)), f / 4, rtol=2e-15)
+    c = np.linspace(1, 8, 32).astype(np.float32)
+    np.testing.assert_allclose(got(H.rope(64, 1e6, freq_factors=c)), f / c.astype(np.float64), rtol=2e-15)
+    # YaRN: pairs that turn often keep their frequency, slow ones are divided
+    corner = lambda t: 64 * math.log(4096 / (2 * math.pi * t)) / (2 * math.log(1e6))  # noqa: E731
+    lo, hi = math.floor(corner(32.0)), math.ceil(corner(1.0))
+    assert 0 < lo < hi < 32
+    r = np.clip((n - lo) / (hi - lo), 0, 1)
+    y = got(H.rope(64, 1e6, factor=8.0, orig_ctx=4096))
+    np.testing.assert_allclose(y, f * (1 - r) + f / 8 * r, rtol=4e-15)
+    assert np.allclose(y[:lo + 1], f[:lo + 1], rtol=2e-15) and np.allclose(y[hi:], f[hi:] / 8, rtol=2e-15)
+    r = H.rope(8, 1e4, layout="interleaved", mscale=1.25)
+    assert r.layout == 1 and r.rot_dim == 8 and r.mscale == 1.25 and r.turns[0] * 2 * math.pi == 1.0
+    assert not any(r.turns[4:])
+
+
+HARNESS = r"""
+#include <cassert>
+#include <climits>
+#include <cstdio>
+#include <initializer_list>
+#include "c2h_paged.h"
+using namespace c2h;
+int main() {
+  // pages: an index is used only inside the pool
+  assert(page_ok(0, 1) && page_ok(99, 100) && !page_ok(100, 100) && !page_ok(-1, 100) && !page_ok(INT_MIN, 100) &&
+         !page_ok(INT_MAX, 100));
+  assert(length_ok(0, 0) && length_ok(5, 5) && !length_ok(6, 5) && !length_ok(-1, 5) && !length_ok(INT_MIN, 1 << 30));
+  // windows and chunks cover the span once, in order, without overflow
+  const int lens[] = {0, 1, 2, 127, 128, 129, 4095, 4096, 100001, 1 << 30};
+  const int wins[] = {0, 1, 127, 128, 1000, 1 << 30};
+  for (int len : lens)
+    for (int w : wins)
+      for (int chunk : {128, 256, 1024}) {
+        const Span s = attended(len, w);
+        assert(s.hi == len && s.lo >= 0 && s.hi - s.lo == (w > 0 && w < len ? w : len));
+        const int n = chunks_of(s, chunk);
+        assert((int64_t)n * chunk >= s.hi - s.lo && (n == 0 || (int64_t)(n - 1) * chunk < s.hi - s.lo));
+        // the pages that a chunk touches fit its table
+        for (int sh = 3; sh <= 10; ++sh)
+          for (int i : {0, n / 2, n - 1}) {
+            if (i < 0 || n == 0) continue;
+            const int64_t c0 = s.lo + (int64_t)i * chunk, c1 = c0 + chunk < s.hi ? c0 + chunk : s.hi;
+            assert(c1 > c0 && ((c1 - 1) >> sh) - (c0 >> sh) + 1 <= ATTN_TAB);
+          }
+      }
+  // the tokens of a session are its last ones
+  assert(token_pos(10, 5, 6) == 9 && token_pos(10, 0, 6) == 4 && token_pos(3, 0, 6) == -3 && token_pos(0, 0, 1) == -1);
+  assert(token_pos(1 << 30, INT_MAX - 1, INT_MAX) == (1 << 30) - 1);
+  // the split: whole chunks, never beyond what a workgroup holds
+  for (int64_t rows : {(int64_t)1, (int64_t)2, (int64_t)14, (int64_t)1000, (int64_t)1 << 24})
+    for (int span : {0, 1, 128, 5000, 1 << 30}) {
+      const int c = attn_chunk(rows, span);
+      assert(c >= 128 && c <= ATTN_MAX_CHUNK && c % 128 == 0);
+    }
+  puts("ok");
+}
+"""
+
+
+def test_index_arithmetic(tmp_path):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(HARNESS)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I",
+                    os.path.join(ROOT, "c2slm_amd", "csrc"), str(src), "-o", str(exe)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout == "ok\n"
+
+
+def test_python_views_refused():
+    class T:
+        def __init__(self, shape, stride):
+            self.shape, self._s, self.ndim = shape, stride, len(shape)
+
+        def stride(self, i=None):
+            return self._s if i is None else self._s[i]
+
+        def data_ptr(self):
+            return A
+
+    with pytest.raises(ValueError):
+        H.heads(T((2, 3, 64), (384, 128, 2)))
+    with pytest.raises(ValueError):
+        H.heads(T((2, 64), (64, 1)))
+    with pytest.raises(ValueError):
+        H.paged_kv(T((4, 16, 2, 64), (2048, 128, 64, 1)), T((4, 16, 2, 64), (4096, 128, 64, 1)), H.BF16)
+    with pytest.raises(ValueError):
+        H.paged_batch(T((3, 4), (4, 1)), T((2,), (1,)), 64)
+    with pytest.raises(ValueError):
+        H.rope(64, 1e6, freq_factors=np.ones(31))
+    p = H.paged_kv(T((4, 2, 16, 64), (2048, 1024, 64, 1)), T((4, 2, 16, 64), (2048, 1024, 64, 1)), H.BF16, order="hnd")
+    assert (p.page_size, p.n_kv_heads, p.token_stride, p.head_stride) == (16, 2, 64, 1024)
