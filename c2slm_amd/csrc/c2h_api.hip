@@ -2558,7 +2558,11 @@ int c2h_gemv(c2h_ctx* c, int32_t type, const void* w, const void* xq, int32_t ro
 namespace {
 
 bool act_type(int t) { return t == C2H_F32 || t == C2H_F16 || t == C2H_BF16; }
-constexpr int64_t kMaxStride = (int64_t)1 << 40;  // elements: offsets stay far inside 64 bits
+// A stride of `count` things, in elements: its offsets stay within 2^48 bytes
+// (no GPU has more), so sums of a few fit 64 bits.
+bool stride_fits(int64_t stride, int64_t count, int es) {
+  return stride >= 0 && stride <= ((int64_t)1 << 48) / es / std::max<int64_t>(count, 1);
+}
 
 // Whether vectors of `dim` elements at the given (stride, count) pairs lie
 // apart: each stride spans everything the smaller ones reach.
@@ -2581,8 +2585,8 @@ int check_heads(c2h_ctx* c, const char* what, const c2h_heads* h, int type, int 
   const int es = type_bytes(type);
   if (n_tokens == 0) return C2H_OK;  // an empty tensor may have no memory
   if (!h || !h->data) return fail(c, C2H_ERR_INVALID, "%s: no data", what);
-  if (h->token_stride < 0 || h->head_stride < 0 || h->token_stride > kMaxStride || h->head_stride > kMaxStride)
-    return fail(c, C2H_ERR_INVALID, "%s: strides from 0 to 2^40 elements", what);
+  if (!stride_fits(h->token_stride, n_tokens, es) || !stride_fits(h->head_stride, n_heads, es))
+    return fail(c, C2H_ERR_INVALID, "%s: strides below 0 or beyond all memory", what);
   if ((reinterpret_cast<uintptr_t>(h->data) | (uintptr_t)(h->token_stride * es) | (uintptr_t)(h->head_stride * es)) & 15)
     return fail(c, C2H_ERR_INVALID, "%s: data and strides must be multiples of 16 bytes", what);
   if (written && !apart({{h->token_stride, n_tokens}, {h->head_stride, n_heads}}, head_dim))
@@ -2608,18 +2612,20 @@ int check_paged(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b) {
   const int es = type_bytes(kv->type);
   if (!kv->k || !kv->v || kv->k == kv->v) return fail(c, C2H_ERR_INVALID, "keys and values need memory of their own");
   const int64_t st[3] = {kv->page_stride, kv->token_stride, kv->head_stride};
+  const int64_t counts[3] = {kv->n_pages, kv->page_size, kv->n_kv_heads};
   uintptr_t low = reinterpret_cast<uintptr_t>(kv->k) | reinterpret_cast<uintptr_t>(kv->v);
-  for (int64_t x : st) {
-    if (x < 0 || x > kMaxStride / 1024) return fail(c, C2H_ERR_INVALID, "cache strides from 0 to 2^30 elements");
-    low |= (uintptr_t)(x * es);
+  for (int i = 0; i < 3; ++i) {
+    if (!stride_fits(st[i], counts[i], es)) return fail(c, C2H_ERR_INVALID, "cache strides below 0 or beyond all memory");
+    low |= (uintptr_t)(st[i] * es);
   }
+  if (kv->token_stride * es > 0x7fffffff) return fail(c, C2H_ERR_UNSUPPORTED, "token_stride beyond 2 GiB");
   if (low & 15) return fail(c, C2H_ERR_INVALID, "cache pointers and strides must be multiples of 16 bytes");
-  if (!apart({{st[0], kv->n_pages}, {st[1], kv->page_size}, {st[2], kv->n_kv_heads}}, kv->head_dim))
+  if (!apart({{st[0], counts[0]}, {st[1], counts[1]}, {st[2], counts[2]}}, kv->head_dim))
     return fail(c, C2H_ERR_INVALID, "cache vectors overlap");
-  if (b->n_seqs < 0 || b->n_seqs > (1 << 20)) return fail(c, C2H_ERR_INVALID, "%d sessions", b->n_seqs);
+  if (b->n_seqs < 0 || b->n_seqs > 65535) return fail(c, C2H_ERR_INVALID, "%d sessions: up to 65535", b->n_seqs);
   if (b->max_len < 0 || b->max_len > (1 << 30)) return fail(c, C2H_ERR_INVALID, "max_len %d", b->max_len);
   if (b->n_seqs > 0 && (!b->block_table || !b->seq_lens)) return fail(c, C2H_ERR_INVALID, "no block table or lengths");
-  if (b->table_stride < 0 || b->table_stride > kMaxStride ||
+  if (!stride_fits(b->table_stride, b->n_seqs, 4) ||
       b->table_stride < ((int64_t)b->max_len + kv->page_size - 1) / kv->page_size)
     return fail(c, C2H_ERR_INVALID, "a table row of %lld pages of %d tokens does not cover max_len %d",
                 (long long)b->table_stride, kv->page_size, b->max_len);
@@ -2671,7 +2677,7 @@ RopeTab rope_tab(const c2h_rope* r) {
 // The launch's shape: workgroups per row, and the workspace their parts meet in.
 int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int n_heads, int window, PagedAttnParams* P,
               size_t* bytes) {
-  if (n_heads < 1 || n_heads > 65536 || n_heads % kv->n_kv_heads)
+  if (n_heads < 1 || n_heads > 4096 || n_heads % kv->n_kv_heads)
     return fail(c, C2H_ERR_INVALID, "%d query heads over %d KV heads", n_heads, kv->n_kv_heads);
   if (window < 0) return fail(c, C2H_ERR_INVALID, "window %d", window);
   P->n_heads = n_heads;
@@ -2680,7 +2686,7 @@ int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int 
   P->window = window;
   const int span = window > 0 ? std::min(window, b->max_len) : b->max_len;
   P->chunk = attn_chunk((int64_t)b->n_seqs * kv->n_kv_heads * P->n_tiles, span);
-  P->n_chunks = std::max(1, chunks_of(Span{0, span}, P->chunk));
+  P->n_chunks = std::max(1, most_chunks(b->max_len, window, P->chunk));
   const int64_t parts = (int64_t)b->n_seqs * n_heads * P->n_chunks;
   if (parts > 0x7fffffff) return fail(c, C2H_ERR_UNSUPPORTED, "%lld parts of rows exceed one launch", (long long)parts);
   *bytes = P->n_chunks > 1 ? (size_t)parts * (kv->head_dim + 2) * 4 : 0;
@@ -2730,7 +2736,7 @@ int c2h_rope_init(const c2h_rope_desc* d, c2h_rope* r) {
 int c2h_rope_dev(c2h_ctx* c, const c2h_rope* rope, int32_t type, const c2h_heads* x, const int32_t* positions,
                  int32_t n_tokens, int32_t n_heads, int32_t head_dim, const c2h_heads* y) {
   if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
-  if (n_tokens < 0 || n_heads < 1 || n_heads > 65536) return fail(c, C2H_ERR_INVALID, "%d tokens of %d heads", n_tokens, n_heads);
+  if (n_tokens < 0 || n_heads < 1 || n_heads > 4096) return fail(c, C2H_ERR_INVALID, "%d tokens of %d heads", n_tokens, n_heads);
   if (head_dim < 8 || head_dim > C2H_ROPE_MAX_DIM || head_dim % 8)
     return fail(c, C2H_ERR_UNSUPPORTED, "head_dim %d: a multiple of 8 up to %d", head_dim, C2H_ROPE_MAX_DIM);
   if (!rope || (n_tokens > 0 && !positions)) return fail(c, C2H_ERR_INVALID, "no rotation or positions");
@@ -2768,7 +2774,7 @@ int c2h_paged_append_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_bat
       (rc = check_heads(c, "v", v, type, n_tokens, kv->n_kv_heads, kv->head_dim, false)))
     return rc;
   if (q || q_out) {
-    if (n_heads < 1 || n_heads > 65536) return fail(c, C2H_ERR_INVALID, "%d query heads", n_heads);
+    if (n_heads < 1 || n_heads > 4096) return fail(c, C2H_ERR_INVALID, "%d query heads", n_heads);
     if ((rc = check_heads(c, "q", q, type, n_tokens, n_heads, kv->head_dim, false)) ||
         (rc = check_heads(c, "q_out", q_out, type, n_tokens, n_heads, kv->head_dim, true)))
       return rc;
@@ -2867,7 +2873,7 @@ int c2h_rmsnorm_q8k_dev(c2h_ctx* c, int32_t type, const void* x, int64_t x_strid
                {y_out, y_stride, 4, true}};
   for (const auto& r : rows) {
     if (!r.p) continue;
-    if (r.stride < 0 || r.stride > kMaxStride || (r.written && n_rows > 1 && r.stride < cols))
+    if (!stride_fits(r.stride, n_rows, r.es) || (r.written && n_rows > 1 && r.stride < cols))
       return fail(c, C2H_ERR_INVALID, "a row stride of %lld elements for %d columns", (long long)r.stride, cols);
     low |= reinterpret_cast<uintptr_t>(r.p) | (uintptr_t)(r.stride * r.es);
   }

@@ -32,8 +32,18 @@ struct Span {
 C2H_HD inline Span attended(int len, int window) {
   return Span{window > 0 && len > window ? len - window : 0, len};
 }
-// Chunks of the span; chunk i is [lo + i * chunk, min(lo + (i+1) * chunk, hi)).
-C2H_HD inline int chunks_of(Span s, int chunk) { return (int)(((int64_t)(s.hi - s.lo) + chunk - 1) / chunk); }
+// The span's chunks begin at multiples of `chunk` from its first position
+// rounded down to a multiple of 4, so that four positions a lane reads
+// together lie in one page; the first chunk's begin at s.lo.
+constexpr int SPAN_ALIGN = 4;
+C2H_HD inline int chunk_base(Span s, int chunk, int i) { return (s.lo & ~(SPAN_ALIGN - 1)) + i * chunk; }
+C2H_HD inline int chunks_of(Span s, int chunk) {
+  return (int)(((int64_t)s.hi - (s.lo & ~(SPAN_ALIGN - 1)) + chunk - 1) / chunk);
+}
+// Chunks of the longest span of a launch: sessions of at most max_len.
+C2H_HD inline int most_chunks(int max_len, int window, int chunk) {
+  return window > 0 && window < max_len ? chunks_of(Span{0, window + SPAN_ALIGN - 1}, chunk) : chunks_of(Span{0, max_len}, chunk);
+}
 
 // Positions per workgroup for a batch of n_rows (session, KV head, head
 // tile) rows whose spans are at most `span`.
@@ -89,14 +99,18 @@ struct RopeTab {
   float mscale;
   double turns[128];
 };
+constexpr int ROPE_TOKENS = 4;  // tokens of a workgroup, one wave's to place each
 struct RopeParams {
-  HeadRows q, qo, k, ko, v;  // ko: rotated keys where there is no cache
+  HeadRows q, qo, k, v;
   PagedKV kv;
   PagedBatch b;
   const int32_t* token_start;
   const int32_t* positions;  // where there is no cache
   int n_tokens, n_q, n_kv;   // heads per token
   int head_dim;
+  int tok;                   // tokens per workgroup
+  int runs;                  // pairs of runs per head, and the divisions by it and by the heads
+  uint32_t runs_magic, rows_magic;
   int* err;
   RopeTab rope;
 };

@@ -2,7 +2,8 @@
 // and its attention (include/c2h.h describes them; none has a counterpart in
 // the reference).
 #include <hip/hip_runtime.h>
-#include <hip/hip_bf16.h>
+
+#include <algorithm>
 
 #include "c2h_paged.h"
 
@@ -12,52 +13,43 @@ namespace {
 
 // ------------------------------------------------------------ element types
 
-template <int T>
-__device__ __forceinline__ float load_as_f32(const char* p, int64_t i) {
-  if constexpr (T == PT_F32) {
-    return reinterpret_cast<const float*>(p)[i];
-  } else if constexpr (T == PT_F16) {
-    return (float)reinterpret_cast<const _Float16*>(p)[i];
-  } else if constexpr (T == PT_BF16) {
-    return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
-  } else {
-    return __builtin_amdgcn_cvt_f32_fp8((int)reinterpret_cast<const uint8_t*>(p)[i], 0);
-  }
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+template <class To, class From>
+__device__ __forceinline__ To as(From v) {
+  return __builtin_bit_cast(To, v);
 }
 
-// Round to nearest even; NaN stays NaN.
-__device__ __forceinline__ uint32_t bf16_bits(float x) {
-  const __bf16 b = (__bf16)x;
-  return (uint32_t)__builtin_bit_cast(uint16_t, b);
-}
-// Saturating: finite values and infinities beyond 448 store as +-448.
-__device__ __forceinline__ uint32_t e4m3_bits(float x) {
-  const float c = x != x ? x : fminf(fmaxf(x, -448.0f), 448.0f);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, c, 0, false) & 0xffu;
-}
-
-template <int T>
-__device__ __forceinline__ void store_f32(char* p, int64_t i, float x) {
-  if constexpr (T == PT_F32) {
-    reinterpret_cast<float*>(p)[i] = x;
-  } else if constexpr (T == PT_F16) {
-    reinterpret_cast<_Float16*>(p)[i] = (_Float16)x;
-  } else if constexpr (T == PT_BF16) {
-    reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)bf16_bits(x);
+// Two floats as 16-bit numbers of the product's type, rounded to nearest even.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (BF) {
+    const bf16x2 v = {(__bf16)a, (__bf16)b};
+    return as<uint32_t>(v);
   } else {
-    reinterpret_cast<uint8_t*>(p)[i] = (uint8_t)e4m3_bits(x);
+    const f16x2 v = {(_Float16)a, (_Float16)b};
+    return as<uint32_t>(v);
   }
 }
-__device__ __forceinline__ float load_type(int t, const char* p, int64_t i) {
-  return t == PT_F32 ? load_as_f32<PT_F32>(p, i) : t == PT_F16 ? load_as_f32<PT_F16>(p, i) : load_as_f32<PT_BF16>(p, i);
+template <bool BF>
+__device__ __forceinline__ float unpack(uint32_t v, int i) {
+  if constexpr (BF) return __uint_as_float(i ? v & 0xffff0000u : v << 16);
+  return (float)as<f16x2>(v)[i];
 }
-__device__ __forceinline__ void store_type(int t, char* p, int64_t i, float x) {
-  if (t == PT_F32)
-    store_f32<PT_F32>(p, i, x);
-  else if (t == PT_F16)
-    store_f32<PT_F16>(p, i, x);
-  else
-    store_f32<PT_BF16>(p, i, x);
+// Saturating: finite values and infinities beyond 448 store as +-448, NaN
+// stays NaN.
+__device__ __forceinline__ float e4m3_range(float x) { return x != x ? x : fminf(fmaxf(x, -448.0f), 448.0f); }
+__device__ __forceinline__ uint32_t e4m3_bits4(float a, float b, float c, float d) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(a), e4m3_range(b), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(c), e4m3_range(d), lo, true);
 }
 
 // Errors are rare: one system-scope or into pinned host memory.
@@ -78,18 +70,20 @@ __device__ __forceinline__ float2 cos_sin(const RopeTab& r, int i, int pos) {
 }
 
 // Where a call's token goes: its position, and the byte offset of its slot
-// in the pool; false if it goes nowhere.
-__device__ bool place(const RopeParams& P, int t, int* pos, int64_t* off) {
+// in the pool; false if it goes nowhere.  One whole wave: its lanes look for
+// the last session that starts at or before t, 64 starts a round.
+__device__ __forceinline__ bool place(const RopeParams& P, int t, int* pos, int64_t* off) {
+  const int lane = threadIdx.x & 63;
   int s = t;
   int64_t end = (int64_t)t + 1;
   if (P.token_start) {
-    int lo = 0, hi = P.b.n_seqs;  // the last session that starts at or before t
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (P.token_start[mid] <= t)
-        lo = mid;
-      else
-        hi = mid;
+    int lo = 0, n = P.b.n_seqs;
+    while (n > 1) {
+      const int step = (n + 63) >> 6;
+      const bool before = lane * step < n && P.token_start[lo + lane * step] <= t;
+      const int skip = max((int)__popcll(__ballot(before)) - 1, 0) * step;
+      lo += skip;
+      n = min(step, n - skip);
     }
     s = lo;
     end = P.token_start[s + 1];
@@ -99,12 +93,12 @@ __device__ bool place(const RopeParams& P, int t, int* pos, int64_t* off) {
   if (len == 0) return false;
   const int64_t p = token_pos(len, t, end);
   if (!length_ok(len, P.b.max_len) || p < 0) {
-    report(P.err, length_ok(len, P.b.max_len) ? PERR_START : PERR_LENGTH);
+    if (lane == 0) report(P.err, length_ok(len, P.b.max_len) ? PERR_START : PERR_LENGTH);
     return false;
   }
   const int page = P.b.table[s * P.b.table_stride + (p >> P.kv.page_shift)];
   if (!page_ok(page, P.kv.n_pages)) {
-    report(P.err, PERR_PAGE);
+    if (lane == 0) report(P.err, PERR_PAGE);
     return false;
   }
   *pos = (int)p;
@@ -112,185 +106,726 @@ __device__ bool place(const RopeParams& P, int t, int* pos, int64_t* off) {
   return true;
 }
 
-// One workgroup per token, a thread per pair (or copied element).
-template <int T, int CT, bool CACHED>
-__global__ void __launch_bounds__(256) k_rope(RopeParams P) {
-  const int t = blockIdx.x;
-  int pos;
-  int64_t off = 0;
-  if constexpr (CACHED) {
-    if (!place(P, t, &pos, &off)) return;
-  } else {
-    pos = P.positions[t];
-  }
-  const RopeTab& R = P.rope;
-  const int half = R.rot_dim / 2, rows = P.n_q + 2 * P.n_kv, per = P.head_dim - half;
-  for (int it = threadIdx.x; it < rows * per; it += 256) {
-    const int row = it / per, i = it % per;
-    const bool is_q = row < P.n_q, is_v = row >= P.n_q + P.n_kv;
-    const int h = is_q ? row : (row - P.n_q) % P.n_kv;
-    const HeadRows& S = is_q ? P.q : is_v ? P.v : P.k;
-    const char* src = S.data + t * S.token_stride + h * S.head_stride;
-    char* dst;
-    float mul = 1.0f;
-    if (is_q)
-      dst = P.qo.data + t * P.qo.token_stride + h * P.qo.head_stride;
-    else if constexpr (CACHED) {
-      dst = (is_v ? P.kv.v : P.kv.k) + off + h * P.kv.head_stride;
-      const float* sc = is_v ? P.kv.v_scale : P.kv.k_scale;
-      if (CT == PT_E4M3 && sc) mul = sc[h];
-    } else
-      dst = P.ko.data + t * P.ko.token_stride + h * P.ko.head_stride;
-    const int a = i < half ? (R.layout == 0 ? i : 2 * i) : i + half, b = i < half ? (R.layout == 0 ? i + half : 2 * i + 1) : a;
-    float x = load_as_f32<T>(src, a), y = load_as_f32<T>(src, b);
-    if (i < half && !is_v) {
-      const float2 cs = cos_sin(R, i, pos);
-      const float u = x * cs.x - y * cs.y, v = x * cs.y + y * cs.x;
-      x = u;
-      y = v;
-    }
-    if (CACHED && !is_q) {
-      store_f32<CT>(dst, a, CT == PT_E4M3 ? x / mul : x);
-      if (b != a) store_f32<CT>(dst, b, CT == PT_E4M3 ? y / mul : y);
+// VEC neighbouring elements as they lie in memory, and as floats.
+template <int T, int VEC>
+struct Run {
+  static constexpr int DW = VEC * type_bytes(T) / 4;
+  uint32_t w[DW];
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (DW % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < DW; i += 4) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(p + 4 * i);
+        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+      }
+    } else if constexpr (DW == 2) {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+      w[0] = v.x, w[1] = v.y;
     } else {
-      store_f32<T>(dst, a, x);
-      if (b != a) store_f32<T>(dst, b, y);
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
     }
+  }
+  __device__ __forceinline__ void store(char* p) const {
+    if constexpr (DW % 4 == 0) {
+#pragma unroll
+      for (int i = 0; i < DW; i += 4) *reinterpret_cast<u32x4*>(p + 4 * i) = u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]};
+    } else if constexpr (DW == 2) {
+      *reinterpret_cast<u32x2*>(p) = u32x2{w[0], w[1]};
+    } else {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = T == PT_F32 ? __uint_as_float(w[i % DW]) : unpack<T == PT_BF16>(w[i / 2 % DW], i & 1);
+  }
+  __device__ __forceinline__ void set(const float (&x)[VEC]) {
+#pragma unroll
+    for (int i = 0; i < DW; ++i) {
+      if constexpr (T == PT_F32)
+        w[i] = __float_as_uint(x[i]);
+      else if constexpr (T == PT_E4M3)
+        w[i] = e4m3_bits4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      else
+        w[i] = pack2<T == PT_BF16>(x[2 * i], x[2 * i + 1]);
+    }
+  }
+};
+
+// A workgroup takes P.tok consecutive tokens, up to four.  Wave w finds token
+// w's place and fills its cosines and sines (one 64-bit angle per pair and
+// token, in LDS for all heads); then every thread moves pairs of VEC-element
+// runs: the two halves of VEC rotated pairs in the half layout, neighbours
+// elsewhere, 16 bytes a load at 16 bits.  The first pair's loads are issued
+// before the angles, which they do not wait for.  Bound by memory: a step of
+// few tokens by its chain of loads (length, page) and the launch.
+template <int T, int CT, bool CACHED, int VEC>
+__global__ void __launch_bounds__(256) k_rope(RopeParams P) {
+  __shared__ float2 cs[ROPE_TOKENS][128];
+  __shared__ int64_t slot[ROPE_TOKENS];  // the token's offset in the pool; < 0: none
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int t0 = blockIdx.x * P.tok, tok = min(P.tok, P.n_tokens - t0);
+  const RopeTab& R = P.rope;
+  const int rows = P.n_q + 2 * P.n_kv, items = tok * rows * P.runs;
+  const int half = R.rot_dim / 2;
+
+  // pair `it` of runs: its token, row, and the elements its runs begin at
+  // (b < 0: only one run)
+  struct Item {
+    int tt, row, a, b;
+    bool turn;
+  };
+  auto item = [&](int it) {
+    Item x;
+    const int q = P.runs == 1 ? it : (int)__umulhi((uint32_t)it, P.runs_magic), c = it - q * P.runs;
+    x.tt = rows == 1 ? q : (int)__umulhi((uint32_t)q, P.rows_magic);
+    x.row = q - x.tt * rows;
+    x.turn = x.row < P.n_q + P.n_kv;
+    const int e = 2 * c * VEC;
+    if (x.turn && R.layout == 0) {
+      x.turn = c * VEC < half;
+      x.a = x.turn ? c * VEC : e;  // half and rot_dim are whole runs: the copied ones go on at 2 c
+      x.b = x.turn ? x.a + half : x.a + VEC;
+    } else {
+      x.a = e;
+      x.b = e + VEC;
+    }
+    if (x.b >= P.head_dim) x.b = -1;
+    return x;
+  };
+  auto source = [&](const Item& x) {
+    const bool is_q = x.row < P.n_q, is_v = x.row >= P.n_q + P.n_kv;
+    const HeadRows& S = is_q ? P.q : is_v ? P.v : P.k;
+    const int h = is_q ? x.row : is_v ? x.row - P.n_q - P.n_kv : x.row - P.n_q;
+    return S.data + (t0 + x.tt) * S.token_stride + h * S.head_stride;
+  };
+  Item x = item(min(tid, items - 1));
+  Run<T, VEC> ra, rb;
+  auto load = [&](const Item& y) {
+    const char* p = source(y);
+    ra.load(p + y.a * type_bytes(T));
+    rb.load(p + max(y.b, 0) * type_bytes(T));
+  };
+  load(x);
+
+  if (wave < tok) {
+    int pos = 0;
+    int64_t off = 0;
+    if constexpr (CACHED) {
+      if (!place(P, t0 + wave, &pos, &off)) off = -1;
+      if (lane == 0) slot[wave] = off;
+    } else {
+      pos = P.positions[t0 + wave];
+    }
+    for (int i = lane; i < half; i += 64) cs[wave][i] = cos_sin(R, i, pos);
+  }
+  __syncthreads();
+
+  for (int it = tid; it < items; it += 256) {
+    float a[VEC], b[VEC];
+    ra.get(a);
+    rb.get(b);
+    const Item y = x;
+    if (it + 256 < items) {
+      x = item(it + 256);
+      load(x);
+    }
+    const float2* c = cs[y.tt];
+    if (y.turn && R.layout == 0) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float2 f = c[y.a + i];
+        const float u = a[i] * f.x - b[i] * f.y, v = a[i] * f.y + b[i] * f.x;
+        a[i] = u;
+        b[i] = v;
+      }
+    } else if (y.turn) {
+      auto turn = [&](float(&z)[VEC], int at) {
+        if (at < 0 || at >= R.rot_dim) return;  // rot_dim is whole runs
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+          const float2 f = c[(at + i) >> 1];
+          const float u = z[i] * f.x - z[i + 1] * f.y, v = z[i] * f.y + z[i + 1] * f.x;
+          z[i] = u;
+          z[i + 1] = v;
+        }
+      };
+      turn(a, y.a);
+      turn(b, y.b);
+    }
+    const bool is_q = y.row < P.n_q, is_v = y.row >= P.n_q + P.n_kv;
+    if constexpr (CACHED) {
+      const int64_t off = slot[y.tt];
+      if (off < 0) continue;
+      if (!is_q) {
+        const int h = is_v ? y.row - P.n_q - P.n_kv : y.row - P.n_q;
+        char* dst = (is_v ? P.kv.v : P.kv.k) + off + h * P.kv.head_stride;
+        if constexpr (CT == PT_E4M3) {
+          const float* sc = is_v ? P.kv.v_scale : P.kv.k_scale;
+          if (sc) {
+            const float d = sc[h];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) a[i] /= d, b[i] /= d;
+          }
+        }
+        Run<CT, VEC> w;
+        w.set(a);
+        w.store(dst + y.a * type_bytes(CT));
+        w.set(b);
+        if (y.b >= 0) w.store(dst + y.b * type_bytes(CT));
+        continue;
+      }
+    }
+    char* dst = P.qo.data + (t0 + y.tt) * P.qo.token_stride + y.row * P.qo.head_stride;
+    Run<T, VEC> w;
+    w.set(a);
+    w.store(dst + y.a * type_bytes(T));
+    w.set(b);
+    if (y.b >= 0) w.store(dst + y.b * type_bytes(T));
   }
 }
 
 // --------------------------------------------------------------- attention
+//
+// One token per session, so every key and value is used once per query head:
+// at 16 heads per KV head 8 operations per byte of a 16-bit pool, far below
+// what the matrix units do per byte of HBM.  The kernel's work is to keep
+// loads in flight, so a wave runs on its own: registers hold its keys and
+// values, nothing of them passes through LDS, and it meets the other waves
+// once, at its end.
+//
+//   scores   S[position][head] = K Q^T: a matrix instruction takes the rows
+//            of K as a lane loads them (16 bytes of one position per lane);
+//            Q lies in LDS in the instruction's order.
+//   softmax  running maximum and sum per head in 32 bits.  S leaves lane l
+//            with head l % 16 and positions 4 (l / 16) + i, which is how the
+//            next product takes P: no value moves between lanes.
+//   output   O^T[dim][head] = V^T P^T.  Lane l loads the same elements
+//            (16 bytes, at l % 16) of the four positions 4 (l / 16) + i, so
+//            its four registers hold a 4-position column of each element, and
+//            the columns that the instruction wants come from byte permutes
+//            within the lane.  Tile t of a row is then every (elements per
+//            lane)-th element, which the epilogue undoes.
+//
+// 16-bit parts: queries and probabilities of 32 bits are split into 16-bit
+// summands (hi = round(x), next = round(x - hi), ...), one matrix
+// instruction each.  Three bf16 or two f16 parts carry 24 and 22 bits: all
+// that 32-bit outputs show.  Two bf16 parts of P (2^-17) stay below a
+// 16-bit output's own rounding.  f16 parts are kept in f16's normal range by
+// powers of two: Q by its head's largest element, P by 2^15 (P <= 1 against
+// the running maximum), which cancels in O / sum.
 
-__device__ __forceinline__ float wg_reduce(float v, float* tmp, bool is_max) {
-  for (int m = 32; m > 0; m >>= 1) {
-    const float o = __shfl_xor(v, m);
-    v = is_max ? fmaxf(v, o) : v + o;
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return is_max ? fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3])) : (tmp[0] + tmp[1]) + (tmp[2] + tmp[3]);
+// The next part of four numbers, which become what it leaves unless it is the
+// last.  An infinite part leaves nothing (rather than the NaN of inf - inf).
+template <bool BF>
+__device__ __forceinline__ u32x2 part4(float (&a)[4], bool last) {
+  const u32x2 v = {pack2<BF>(a[0], a[1]), pack2<BF>(a[2], a[3])};
+  if (!last)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = __builtin_isinf(a[i]) ? 0.0f : a[i] - unpack<BF>(v[i >> 1], i & 1);
+  return v;
 }
 
-// One workgroup per (chunk, query head, session): scores of the chunk by a
-// thread per position, then the weighted sum by a thread per element.
-template <int CT>
-__global__ void __launch_bounds__(256) k_paged_attn(PagedAttnParams P) {
-  __shared__ float sc[ATTN_MAX_CHUNK], qs[256], tmp[4];
-  __shared__ int tab[ATTN_TAB], bad;
-  const int chunk = blockIdx.x % P.n_chunks, head = blockIdx.x / P.n_chunks % P.n_heads, s = blockIdx.x / P.n_chunks / P.n_heads;
-  const int tid = threadIdx.x, hd = P.kv.head_dim, kvh = head / P.group;
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as<bf16x8>(a), as<bf16x8>(b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(as<f16x8>(a), as<f16x8>(b), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma16(u32x2 a, u32x2 b, f32x4 c) {
+  if constexpr (BF) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(as<i16x4>(a), as<i16x4>(b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(as<f16x4>(a), as<f16x4>(b), c, 0, 0, 0);
+}
+
+// Four e4m3 as four f16 (exact).
+__device__ __forceinline__ u32x2 e4m3_to_f16(uint32_t v) {
+  return u32x2{as<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)v, 1.0f, false)),
+               as<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)v, 1.0f, true))};
+}
+
+// Over the four lanes l % 16 of a wave.
+__device__ __forceinline__ float max_of_rows(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_of_rows(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+__device__ __forceinline__ f32x4 load4(int t, const char* p) {
+  if (t == PT_F32) return *reinterpret_cast<const f32x4*>(p);
+  const u32x2 u = *reinterpret_cast<const u32x2*>(p);
+  if (t == PT_BF16) return f32x4{unpack<true>(u.x, 0), unpack<true>(u.x, 1), unpack<true>(u.y, 0), unpack<true>(u.y, 1)};
+  return f32x4{unpack<false>(u.x, 0), unpack<false>(u.x, 1), unpack<false>(u.y, 0), unpack<false>(u.y, 1)};
+}
+__device__ __forceinline__ void store4(int t, char* p, f32x4 v) {
+  if (t == PT_F32)
+    *reinterpret_cast<f32x4*>(p) = v;
+  else if (t == PT_BF16)
+    *reinterpret_cast<u32x2*>(p) = u32x2{pack2<true>(v.x, v.y), pack2<true>(v.z, v.w)};
+  else
+    *reinterpret_cast<u32x2*>(p) = u32x2{pack2<false>(v.x, v.y), pack2<false>(v.z, v.w)};
+}
+
+// exp2(m - mu) where m may be -inf (nothing summed: 0).
+__device__ __forceinline__ float weight(float m, float mu) { return __builtin_amdgcn_exp2f(m - mu); }
+__device__ __forceinline__ float finite_max(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+
+constexpr float MINUS_INF = -__builtin_inff();
+
+// CT: the pool's type; HD: head_dim rounded up to 64, 128 or 256; FULL:
+// head_dim == HD; PRECISE: the 32-bit split above (for outputs or queries
+// that need it).
+template <int CT, int HD, bool FULL, bool PRECISE>
+struct Attn {
+  static constexpr int ES = type_bytes(CT);
+  static constexpr bool F32 = CT == PT_F32, BF = CT == PT_BF16, F8 = CT == PT_E4M3;
+  static constexpr int KC = HD * ES / 64;              // 16-byte loads of a key per lane
+  static constexpr int VB = HD * ES / 16 < 16 ? HD * ES / 16 : 16;  // bytes of a value load
+  static constexpr int VW = VB / 4, VE = VB / ES;      // its dwords, its elements
+  static constexpr int NV = HD * ES / 16 / VB;         // loads of a value per lane
+  static constexpr int NO = HD / 16;                   // output tiles: NV * VE
+  // tiles of 16 positions per step: 16 KB of keys and values per wave (f32
+  // of 256: 32 KB)
+  static constexpr int NT = 256 / (HD * ES) < 1 ? 1 : 512 / (HD * ES) < 1 ? 1 : 512 / (HD * ES);
+  static constexpr int STEP = 16 * NT;
+  static constexpr int NQ = F32 ? 1 : PRECISE ? (BF ? 3 : 2) : 1;
+  static constexpr int NP = F32 ? 1 : BF && PRECISE ? 3 : 2;
+  static constexpr int FR = F32 ? HD / 16 : HD / 32;   // 16-byte fragments of a query per lane
+  static constexpr float BIAS = F32 || BF ? 0.0f : 15.0f;
+  static constexpr int DB = HD < 128 ? HD : 128;       // elements that waves join at a time
+  static constexpr int OROW = DB + 4;
+  static constexpr int Q_BYTES = NQ * FR * 1024, O_BYTES = 4 * 16 * OROW * 4;
+  static constexpr int LDS = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
+};
+
+template <int CT, int HD, bool FULL, bool PRECISE>
+__global__ void __launch_bounds__(256, (CT == PT_F32 && HD == 256) ? 1 : 2) k_paged_attn(PagedAttnParams P) {
+  using A = Attn<CT, HD, FULL, PRECISE>;
+  constexpr int KC = A::KC, NT = A::NT, NV = A::NV, VW = A::VW, VE = A::VE, NO = A::NO, FR = A::FR, NQ = A::NQ, NP = A::NP;
+  constexpr bool BF = A::BF;
+  __shared__ __align__(16) char lds[A::LDS];
+  __shared__ int64_t tab[ATTN_TAB];  // the pages' offsets in the pool
+  __shared__ int bad;
+  __shared__ float mul[16], wm[4][16], wl[4][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, j = lane >> 4;
+  const int chunk = blockIdx.x, s = blockIdx.z;
+  const int kvh = blockIdx.y / P.n_tiles, h0 = kvh * P.group + (blockIdx.y - kvh * P.n_tiles) * ATTN_HEADS;
+  const int nh = min(ATTN_HEADS, (kvh + 1) * P.group - h0);
+  const int hd = FULL ? HD : P.kv.head_dim, shift = P.kv.page_shift;
+
   const int len = P.b.lens[s];
   const bool ok = length_ok(len, P.b.max_len);
   const Span span = attended(ok ? len : 0, P.window);
   const int n = max(chunks_of(span, P.chunk), 1);
   if (chunk >= n) return;
-  const int c0 = span.lo + chunk * P.chunk, c1 = min(c0 + P.chunk, span.hi), p0 = c0 >> P.kv.page_shift;
-  if (tid == 0) bad = 0;
+  const int base0 = chunk_base(span, P.chunk, chunk), c0 = max(base0, span.lo), c1 = min(base0 + P.chunk, span.hi);
+  const int p0 = c0 >> shift;
+
+  // the chunk's pages, and the queries split into the parts of the product
+  if (tid == 0) bad = !ok;
   __syncthreads();
-  if (c1 > c0)
-    for (int i = tid; i <= ((c1 - 1) >> P.kv.page_shift) - p0; i += 256) {
-      tab[i] = P.b.table[s * P.b.table_stride + p0 + i];
-      if (!page_ok(tab[i], P.kv.n_pages)) bad = 1;
+  for (int i = tid; i <= ((c1 - 1) >> shift) - p0 && c1 > c0; i += 256) {
+    const int page = P.b.table[s * P.b.table_stride + p0 + i];
+    tab[i] = page * P.kv.page_stride + kvh * P.kv.head_stride;
+    if (!page_ok(page, P.kv.n_pages)) bad = 2;
+  }
+  {
+    constexpr int EPT = HD / 16;  // elements per thread
+    const int head = tid >> 4, d0 = (tid & 15) * EPT;
+    f32x4 q[EPT / 4];
+#pragma unroll
+    for (int g = 0; g < EPT / 4; ++g) {
+      const bool have = head < nh && (FULL || d0 + 4 * g < hd);
+      q[g] = have ? load4(P.type, P.q.data + s * P.q.token_stride + (h0 + head) * P.q.head_stride +
+                                      (int64_t)(d0 + 4 * g) * (P.type == PT_F32 ? 4 : 2))
+                  : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-  for (int d = tid; d < hd; d += 256)
-    qs[d] = load_type(P.type, P.q.data + s * P.q.token_stride + head * P.q.head_stride, d);
+    int e = 0;
+    if constexpr (A::BIAS != 0.0f) {
+      float top = 0.0f;
+#pragma unroll
+      for (int g = 0; g < EPT / 4; ++g)
+        top = fmaxf(fmaxf(top, fmaxf(fabsf(q[g].x), fabsf(q[g].y))), fmaxf(fabsf(q[g].z), fabsf(q[g].w)));
+#pragma unroll
+      for (int m = 1; m < 16; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+      if (top > 0.0f && top < __builtin_inff()) {
+        e = 14 + 127 - (int)(__float_as_uint(top) >> 23);
+        e = min(max(e, -115), 100);
+      }
+    }
+    if ((tid & 15) == 0) {
+      const float ks = A::F8 && P.kv.k_scale ? P.kv.k_scale[kvh] : 1.0f;
+      mul[head] = ldexpf(P.scale_log2 * ks, -e);
+    }
+#pragma unroll
+    for (int g = 0; g < EPT / 4; ++g) {
+      const int d = d0 + 4 * g;
+      if constexpr (A::F32) {
+        *reinterpret_cast<f32x4*>(lds + ((d >> 4) * 64 + ((d >> 2) & 3) * 16 + head) * 16) = q[g];
+      } else {
+        const int f = A::F8 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5, jj = A::F8 ? (d >> 4) & 3 : (d >> 3) & 3;
+        char* at = lds + (f * 64 + jj * 16 + head) * 16 + ((d >> 2) & 1) * 8;
+        float a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = A::BIAS != 0.0f ? ldexpf(q[g][i], e) : q[g][i];
+#pragma unroll
+        for (int p = 0; p < NQ; ++p) {
+          *reinterpret_cast<u32x2*>(at + p * FR * 1024) = part4<BF>(a, p + 1 == NQ);
+        }
+      }
+    }
+  }
   __syncthreads();
-  char* out = P.out.data + s * P.out.token_stride + head * P.out.head_stride;
-  const bool fail = bad || !ok;
-  float m = -__builtin_inff(), l = 0.0f;
-  if (!fail) {
-    const float ks = CT == PT_E4M3 && P.kv.k_scale ? P.kv.k_scale[kvh] : 1.0f;
-    auto slot = [&](int p) {
-      return tab[(p >> P.kv.page_shift) - p0] * P.kv.page_stride + (p & ((1 << P.kv.page_shift) - 1)) * P.kv.token_stride +
-             kvh * P.kv.head_stride;
+  const bool fail = bad != 0;
+  const float smul = mul[r];
+
+  f32x4 o[NO];
+#pragma unroll
+  for (int t = 0; t < NO; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = MINUS_INF, l = 0.0f;
+
+  if (!fail && base0 + wave * A::STEP < c1) {
+    u32x4 K[NT][KC];
+    uint32_t V[NT][4][NV][VW];
+    const int rowb = hd * A::ES, mask = (1 << shift) - 1, last = c1 - 1;
+    const uint32_t ts = (uint32_t)P.kv.token_stride;  // below 2^31
+    // Positions outside [c0, c1) are read as the nearest inside, and masked
+    // in the scores; elements past head_dim as the row's first, against zeros
+    // of Q and into output tiles that are not stored.
+    auto inside = [&](int pos) { return min(max(pos, c0), last); };
+    auto page_of = [&](int pos) { return tab[(pos >> shift) - p0]; };
+    auto in_page = [&](int pos) { return (int64_t)((uint64_t)(uint32_t)(pos & mask) * ts); };
+    auto load_k = [&](int base) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int pos = inside(base + 16 * t + r);
+        const char* row = P.kv.k + page_of(pos) + in_page(pos);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          int off = c * 64 + j * 16;
+          if constexpr (!FULL) off = off < rowb ? off : 0;
+          K[t][c] = *reinterpret_cast<const u32x4*>(row + off);
+        }
+      }
     };
-    for (int p = c0 + tid; p < c1; p += 256) {
-      const char* row = P.kv.k + slot(p);
-      float a = 0.0f;
-      for (int d = 0; d < hd; ++d) a = __builtin_fmaf(qs[d], load_as_f32<CT>(row, d), a);
-      sc[p - c0] = a * (P.scale_log2 * ks);
-      m = fmaxf(m, sc[p - c0]);
+    auto load_v = [&](int base) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        // one page holds those of the four positions that are inside
+        const int first = base + 16 * t + 4 * j;
+        const char* page = P.kv.v + page_of(inside(first));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const char* row = page + in_page(inside(first + i));
+#pragma unroll
+          for (int b = 0; b < NV; ++b) {
+            int off = b * 16 * A::VB + r * A::VB;
+            if constexpr (!FULL) off = off < rowb ? off : 0;
+            if constexpr (VW == 4) {
+              const u32x4 v = *reinterpret_cast<const u32x4*>(row + off);
+#pragma unroll
+              for (int w = 0; w < 4; ++w) V[t][i][b][w] = v[w];
+            } else if constexpr (VW == 2) {
+              const u32x2 v = *reinterpret_cast<const u32x2*>(row + off);
+              V[t][i][b][0] = v.x;
+              V[t][i][b][1] = v.y;
+            } else {
+              V[t][i][b][0] = *reinterpret_cast<const uint32_t*>(row + off);
+            }
+          }
+        }
+      }
+    };
+    load_k(base0 + wave * A::STEP);
+    load_v(base0 + wave * A::STEP);
+    for (int base = base0 + wave * A::STEP; base < c1; base += 4 * A::STEP) {
+      const int next = base + 4 * A::STEP;
+      // scores
+      f32x4 S[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) S[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int p = 0; p < NQ; ++p)
+#pragma unroll
+        for (int f = 0; f < FR; ++f) {
+          const u32x4 q = *reinterpret_cast<const u32x4*>(lds + ((p * FR + f) * 64 + lane) * 16);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            if constexpr (A::F32) {
+              const f32x4 a = as<f32x4>(K[t][f]), b = as<f32x4>(q);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], S[t], 0, 0, 0);
+            } else if constexpr (A::F8) {
+              const u32x2 lo = e4m3_to_f16(K[t][f / 2][(f & 1) * 2]), hi = e4m3_to_f16(K[t][f / 2][(f & 1) * 2 + 1]);
+              S[t] = mfma32<BF>(u32x4{lo.x, lo.y, hi.x, hi.y}, q, S[t]);
+            } else {
+              S[t] = mfma32<BF>(K[t][f], q, S[t]);
+            }
+          }
+        }
+      load_k(next);
+      // softmax
+      const uint32_t at = (uint32_t)(base + 4 * j - c0), held = (uint32_t)(c1 - c0);
+      float top = MINUS_INF;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          S[t][i] = at + (16 * t + i) < held ? S[t][i] * smul : MINUS_INF;
+          top = fmaxf(top, S[t][i]);
+        }
+      if (__any(top > m)) {
+        const float mn = fmaxf(m, max_of_rows(top)), a = weight(m, finite_max(mn));
+        m = mn;
+        l *= a;
+#pragma unroll
+        for (int t = 0; t < NO; ++t) o[t] *= a;
+      }
+      const float mb = finite_max(m) - A::BIAS;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          S[t][i] = __builtin_amdgcn_exp2f(S[t][i] - mb);
+          l += S[t][i];
+        }
+      // output
+      if constexpr (A::F32) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int b = 0; b < NV; ++b)
+#pragma unroll
+              for (int w = 0; w < VW; ++w)
+                o[b * VE + w] =
+                    __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(V[t][i][b][w]), S[t][i], o[b * VE + w], 0, 0, 0);
+      } else {
+        u32x2 p[NT][NP];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float a[4] = {S[t][0], S[t][1], S[t][2], S[t][3]};
+#pragma unroll
+          for (int q = 0; q < NP; ++q) p[t][q] = part4<BF>(a, q + 1 == NP);
+        }
+#pragma unroll
+        for (int b = 0; b < NV; ++b)
+#pragma unroll
+          for (int w = 0; w < VE / 2; ++w) {  // elements 2w and 2w + 1 of the load
+            u32x2 col[NT][2];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              uint32_t x[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if constexpr (A::F8)
+                  x[i] = e4m3_to_f16(V[t][i][b][w / 2])[w & 1];
+                else
+                  x[i] = V[t][i][b][w];
+              }
+              col[t][0] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u)};
+              col[t][1] = u32x2{__builtin_amdgcn_perm(x[1], x[0], 0x07060302u), __builtin_amdgcn_perm(x[3], x[2], 0x07060302u)};
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              f32x4& acc = o[b * VE + 2 * w + h];
+#pragma unroll
+              for (int q = 0; q < NP; ++q) {
+                if constexpr (NT % 2 == 0) {
+#pragma unroll
+                  for (int t = 0; t < NT; t += 2)
+                    acc = mfma32<BF>(u32x4{col[t][h].x, col[t][h].y, col[t + 1][h].x, col[t + 1][h].y},
+                                     u32x4{p[t][q].x, p[t][q].y, p[t + 1][q].x, p[t + 1][q].y}, acc);
+                } else {
+#pragma unroll
+                  for (int t = 0; t < NT; ++t) acc = mfma16<BF>(col[t][h], p[t][q], acc);
+                }
+              }
+            }
+          }
+      }
+      load_v(next);
     }
-    m = wg_reduce(m, tmp, true);
-    const float mu = m == -__builtin_inff() ? 0.0f : m;
-    for (int p = c0 + tid; p < c1; p += 256) {
-      sc[p - c0] = __builtin_amdgcn_exp2f(sc[p - c0] - mu);
-      l += sc[p - c0];
+    l = sum_of_rows(l);
+  }
+
+  // the waves' sums, brought to their common maximum, DB elements at a time
+  if (lane < 16) {
+    wm[wave][r] = m;
+    wl[wave][r] = l;
+  }
+  float* os = reinterpret_cast<float*>(lds);
+  const float vs = A::F8 && P.kv.v_scale ? P.kv.v_scale[kvh] : 1.0f;
+#pragma unroll
+  for (int d0 = 0; d0 < HD; d0 += A::DB) {
+    __syncthreads();  // the queries, or the elements before, are read
+    if (r < nh) {
+#pragma unroll
+      for (int t = 0; t < NO; t += 4) {
+        // tiles t .. t+3 of load b: elements row * VE + t % VE + 0 .. 3 of its 16 VE
+        const int b = t / VE;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = b * 16 * VE + (4 * j + i) * VE + t % VE - d0;
+          if (d >= 0 && d < A::DB)
+            *reinterpret_cast<f32x4*>(os + (wave * 16 + r) * A::OROW + d) =
+                f32x4{o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]};
+        }
+      }
     }
-    l = wg_reduce(l, tmp, false);
     __syncthreads();
-    for (int d = tid; d < hd; d += 256) {
-      float a = 0.0f;
-      for (int p = c0; p < c1; ++p) a = __builtin_fmaf(sc[p - c0], load_as_f32<CT>(P.kv.v + slot(p), d), a);
-      const float vs = CT == PT_E4M3 && P.kv.v_scale ? P.kv.v_scale[kvh] : 1.0f;
-      if (n == 1)
-        store_type(P.type, out, d, l == 0.0f ? 0.0f : a / l * vs);
-      else
-        P.part_o[(((int64_t)s * P.n_heads + head) * P.n_chunks + chunk) * hd + d] = a * vs;
-    }
-  } else {
-    if (tid == 0) report(P.err, ok ? PERR_PAGE : PERR_LENGTH);
-    for (int d = tid; d < hd; d += 256) {
-      if (n == 1)
-        store_type(P.type, out, d, __builtin_nanf(""));
-      else
-        P.part_o[(((int64_t)s * P.n_heads + head) * P.n_chunks + chunk) * hd + d] = __builtin_nanf("");
+    for (int it = tid; it < nh * (A::DB / 4); it += 256) {
+      const int head = it / (A::DB / 4), d = (it % (A::DB / 4)) * 4;
+      if (!FULL && d0 + d >= hd) continue;
+      const float top = fmaxf(fmaxf(wm[0][head], wm[1][head]), fmaxf(wm[2][head], wm[3][head])), mu = finite_max(top);
+      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float a = weight(wm[w][head], mu);
+        total += wl[w][head] * a;
+        sum += *reinterpret_cast<const f32x4*>(os + (w * 16 + head) * A::OROW + d) * a;
+      }
+      if (fail) sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f} + __builtin_nanf("");
+      const int64_t row = (int64_t)s * P.n_heads + h0 + head;
+      if (n == 1) {
+        const float inv = fail ? 1.0f : total == 0.0f ? 0.0f : vs / total;
+        store4(P.type, P.out.data + s * P.out.token_stride + (h0 + head) * P.out.head_stride +
+                           (int64_t)(d0 + d) * (P.type == PT_F32 ? 4 : 2), sum * inv);
+      } else {
+        *reinterpret_cast<f32x4*>(P.part_o + (row * P.n_chunks + chunk) * hd + d0 + d) = sum * vs;
+        if (d0 + d == 0) {
+          P.part_ml[(row * P.n_chunks + chunk) * 2] = top;
+          P.part_ml[(row * P.n_chunks + chunk) * 2 + 1] = total;
+        }
+      }
     }
   }
-  if (n > 1 && tid == 0) {
-    float* ml = P.part_ml + (((int64_t)s * P.n_heads + head) * P.n_chunks + chunk) * 2;
-    ml[0] = m;
-    ml[1] = l;
-  }
+  if (fail && tid == 0) report(P.err, ok ? PERR_PAGE : PERR_LENGTH);
 }
 
-// Joins the chunks of a row: the sums brought to the common maximum.
+// Joins the chunks of a row: the sums brought to the common maximum.  One
+// workgroup per row; HDP / 4 threads hold the row's elements, 1024 / HDP
+// groups of them every so-manieth chunk each.
+template <int HDP>
 __global__ void __launch_bounds__(256) k_paged_join(PagedAttnParams P) {
-  const int head = blockIdx.x % P.n_heads, s = blockIdx.x / P.n_heads, hd = P.kv.head_dim;
+  constexpr int LANES = HDP / 4, GROUPS = 256 / LANES;
+  __shared__ float tmp[4];
+  __shared__ __align__(16) float part[GROUPS][HDP + 4];
+  const int head = blockIdx.x, s = blockIdx.y, hd = P.kv.head_dim, tid = threadIdx.x;
   const int len = P.b.lens[s];
   const int n = chunks_of(attended(length_ok(len, P.b.max_len) ? len : 0, P.window), P.chunk);
   if (n <= 1) return;
   const int64_t row = ((int64_t)s * P.n_heads + head) * P.n_chunks;
-  float m = -__builtin_inff(), l = 0.0f;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, P.part_ml[(row + i) * 2]);
-  const float mu = m == -__builtin_inff() ? 0.0f : m;
-  for (int i = 0; i < n; ++i) l += P.part_ml[(row + i) * 2 + 1] * __builtin_amdgcn_exp2f(P.part_ml[(row + i) * 2] - mu);
-  for (int d = threadIdx.x; d < hd; d += 256) {
-    float a = 0.0f;
-    for (int i = 0; i < n; ++i)
-      a += P.part_o[(row + i) * hd + d] * __builtin_amdgcn_exp2f(P.part_ml[(row + i) * 2] - mu);
-    store_type(P.type, P.out.data + s * P.out.token_stride + head * P.out.head_stride, d, l == 0.0f ? a * 0.0f : a / l);
+  const float2* ml = reinterpret_cast<const float2*>(P.part_ml) + row;
+  float m = MINUS_INF;
+  for (int i = tid; i < n; i += 256) m = fmaxf(m, ml[i].x);
+  for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+  if ((tid & 63) == 0) tmp[tid >> 6] = m;
+  __syncthreads();
+  const float mu = finite_max(fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3])));
+  const int g = tid / LANES, d = (tid % LANES) * 4;
+  f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+  float l = 0.0f;
+  for (int i = g; i < n; i += GROUPS) {
+    const float w = weight(ml[i].x, mu);
+    l += ml[i].y * w;
+    if (d < hd) a += *reinterpret_cast<const f32x4*>(P.part_o + (row + i) * hd + d) * w;
   }
+  *reinterpret_cast<f32x4*>(&part[g][d]) = a;
+  if (d == 0) part[g][HDP] = l;
+  __syncthreads();
+  if (g == 0 && d < hd) {
+    l = 0.0f;
+    a = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      a += *reinterpret_cast<const f32x4*>(&part[i][d]);
+      l += part[i][HDP];
+    }
+    // no weight at all: zeros, but the NaN of a bad table stays
+    store4(P.type, P.out.data + s * P.out.token_stride + head * P.out.head_stride + (int64_t)d * (P.type == PT_F32 ? 4 : 2),
+           l == 0.0f ? a * 0.0f : a / l);
+  }
+}
+
+template <int CT, int HD, bool FULL, bool PRECISE>
+void launch_attn_as(const PagedAttnParams& P, hipStream_t st) {
+  const dim3 grid(P.n_chunks, P.kv.n_kv_heads * P.n_tiles, P.b.n_seqs);
+  hipLaunchKernelGGL((k_paged_attn<CT, HD, FULL, PRECISE>), grid, dim3(256), 0, st, P);
+  if (P.n_chunks > 1) hipLaunchKernelGGL(k_paged_join<HD>, dim3(P.n_heads, P.b.n_seqs), dim3(256), 0, st, P);
+}
+
+// Queries and outputs that a single 16-bit part holds take the shorter
+// split: the pool's own type, and either 16-bit type on f16 and e4m3 pools
+// (a bf16 query fits f16's bits once its range is brought in).
+template <int CT, int HD>
+void launch_attn_hd(const PagedAttnParams& P, hipStream_t st) {
+  if (P.kv.head_dim != HD) return launch_attn_as<CT, HD, false, true>(P, st);
+  if constexpr (CT != PT_F32) {
+    if (CT == PT_BF16 ? P.type == PT_BF16 : P.type != PT_F32) return launch_attn_as<CT, HD, true, false>(P, st);
+  }
+  launch_attn_as<CT, HD, true, true>(P, st);
+}
+template <int CT>
+void launch_attn_t(const PagedAttnParams& P, hipStream_t st) {
+  if (P.kv.head_dim <= 64)
+    launch_attn_hd<CT, 64>(P, st);
+  else if (P.kv.head_dim <= 128)
+    launch_attn_hd<CT, 128>(P, st);
+  else
+    launch_attn_hd<CT, 256>(P, st);
 }
 
 }  // namespace
 
 void launch_paged_attn(const PagedAttnParams& P, int cache_type, hipStream_t st) {
-  const dim3 grid(P.n_chunks * P.n_heads * P.b.n_seqs), block(256);
   switch (cache_type) {
-    case PT_F32: hipLaunchKernelGGL(k_paged_attn<PT_F32>, grid, block, 0, st, P); break;
-    case PT_F16: hipLaunchKernelGGL(k_paged_attn<PT_F16>, grid, block, 0, st, P); break;
-    case PT_BF16: hipLaunchKernelGGL(k_paged_attn<PT_BF16>, grid, block, 0, st, P); break;
-    default: hipLaunchKernelGGL(k_paged_attn<PT_E4M3>, grid, block, 0, st, P); break;
+    case PT_F32: launch_attn_t<PT_F32>(P, st); break;
+    case PT_F16: launch_attn_t<PT_F16>(P, st); break;
+    case PT_BF16: launch_attn_t<PT_BF16>(P, st); break;
+    default: launch_attn_t<PT_E4M3>(P, st); break;
   }
-  if (P.n_chunks > 1) hipLaunchKernelGGL(k_paged_join, dim3(P.n_heads * P.b.n_seqs), block, 0, st, P);
 }
 
 namespace {
+template <int T, int CT, bool CACHED>
+void launch_rope_as(RopeParams P, hipStream_t st) {
+  // the halves of a rotated head are whole runs of 8 elements, or of 4
+  const bool narrow = P.rope.layout == 0 && P.rope.rot_dim % 16 != 0;
+  const int vec = narrow ? 4 : 8;
+  const int rows = P.n_q + 2 * P.n_kv;
+  P.runs = (P.head_dim / vec + 1) / 2;
+  // x / d = (x * ceil(2^32 / d)) >> 32 for x up to 4 * rows * runs, far below 2^32 / d
+  P.runs_magic = (uint32_t)(((1ull << 32) + P.runs - 1) / P.runs);
+  P.rows_magic = (uint32_t)(((1ull << 32) + rows - 1) / rows);
+  // more tokens to a workgroup once there are enough workgroups without
+  P.tok = std::min(std::max(P.n_tokens / 1024, 1), ROPE_TOKENS);
+  const dim3 grid((P.n_tokens + P.tok - 1) / P.tok);
+  if (narrow)
+    hipLaunchKernelGGL((k_rope<T, CT, CACHED, 4>), grid, dim3(256), 0, st, P);
+  else
+    hipLaunchKernelGGL((k_rope<T, CT, CACHED, 8>), grid, dim3(256), 0, st, P);
+}
 template <int T>
 void launch_rope_t(const RopeParams& P, int cache_type, bool cached, hipStream_t st) {
-  const dim3 grid(P.n_tokens), block(256);
   if (!cached)
-    hipLaunchKernelGGL((k_rope<T, T, false>), grid, block, 0, st, P);
+    launch_rope_as<T, T, false>(P, st);
   else if (cache_type == PT_F32)
-    hipLaunchKernelGGL((k_rope<T, PT_F32, true>), grid, block, 0, st, P);
+    launch_rope_as<T, PT_F32, true>(P, st);
   else if (cache_type == PT_F16)
-    hipLaunchKernelGGL((k_rope<T, PT_F16, true>), grid, block, 0, st, P);
+    launch_rope_as<T, PT_F16, true>(P, st);
   else if (cache_type == PT_BF16)
-    hipLaunchKernelGGL((k_rope<T, PT_BF16, true>), grid, block, 0, st, P);
+    launch_rope_as<T, PT_BF16, true>(P, st);
   else
-    hipLaunchKernelGGL((k_rope<T, PT_E4M3, true>), grid, block, 0, st, P);
+    launch_rope_as<T, PT_E4M3, true>(P, st);
 }
 }  // namespace
 
