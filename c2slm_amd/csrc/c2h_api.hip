@@ -2623,7 +2623,7 @@ int check_paged(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b) {
   if (!apart({{st[0], counts[0]}, {st[1], counts[1]}, {st[2], counts[2]}}, kv->head_dim))
     return fail(c, C2H_ERR_INVALID, "cache vectors overlap");
   if (b->n_seqs < 0 || b->n_seqs > 65535) return fail(c, C2H_ERR_INVALID, "%d sessions: up to 65535", b->n_seqs);
-  if (b->max_len < 0 || b->max_len > (1 << 30)) return fail(c, C2H_ERR_INVALID, "max_len %d", b->max_len);
+  if (b->max_len < 0 || b->max_len > PAGED_MAX_LEN) return fail(c, C2H_ERR_INVALID, "max_len %d", b->max_len);
   if (b->n_seqs > 0 && (!b->block_table || !b->seq_lens)) return fail(c, C2H_ERR_INVALID, "no block table or lengths");
   if (!stride_fits(b->table_stride, b->n_seqs, 4) ||
       b->table_stride < ((int64_t)b->max_len + kv->page_size - 1) / kv->page_size)
@@ -2674,9 +2674,10 @@ RopeTab rope_tab(const c2h_rope* r) {
   return t;
 }
 
-// The launch's shape: workgroups per row, and the workspace their parts meet in.
+// The launch's shape, and the workspace that chunks of a row meet in: parts
+// (chunk, head) sums, and the sessions' places among them.
 int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int n_heads, int window, PagedAttnParams* P,
-              size_t* bytes) {
+              size_t* bytes, int64_t* parts) {
   if (n_heads < 1 || n_heads > 4096 || n_heads % kv->n_kv_heads)
     return fail(c, C2H_ERR_INVALID, "%d query heads over %d KV heads", n_heads, kv->n_kv_heads);
   if (window < 0) return fail(c, C2H_ERR_INVALID, "window %d", window);
@@ -2684,12 +2685,17 @@ int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int 
   P->group = n_heads / kv->n_kv_heads;
   P->n_tiles = (P->group + ATTN_HEADS - 1) / ATTN_HEADS;
   P->window = window;
-  const int span = window > 0 ? std::min(window, b->max_len) : b->max_len;
-  P->chunk = attn_chunk((int64_t)b->n_seqs * kv->n_kv_heads * P->n_tiles, span);
-  P->n_chunks = std::max(1, most_chunks(b->max_len, window, P->chunk));
-  const int64_t parts = (int64_t)b->n_seqs * n_heads * P->n_chunks;
-  if (parts > 0x7fffffff) return fail(c, C2H_ERR_UNSUPPORTED, "%lld parts of rows exceed one launch", (long long)parts);
-  *bytes = P->n_chunks > 1 ? (size_t)parts * (kv->head_dim + 2) * 4 : 0;
+  P->n_rows = kv->n_kv_heads * P->n_tiles;
+  const int unit = attn_unit(kv->type, kv->head_dim);
+  P->most = most_units(unit, kv->page_size);
+  // a window's first position may add up to three to its span
+  const int span = window > 0 && window < b->max_len ? window + SPAN_ALIGN - 1 : b->max_len;
+  const int64_t chunks = chunks_bound(b->n_seqs, P->n_rows, units_of(Span{0, span}, unit), P->most);
+  if (chunks * n_heads > 0x7fffffff)
+    return fail(c, C2H_ERR_UNSUPPORTED, "%lld chunks of %d heads exceed one launch", (long long)chunks, n_heads);
+  P->grid = (int)std::min<int64_t>(chunks * P->n_rows, ATTN_WGS);
+  *parts = span > unit ? chunks * n_heads : 0;
+  *bytes = *parts ? (size_t)*parts * (kv->head_dim + 2) * 4 + (size_t)b->n_seqs * 8 : 0;
   return C2H_OK;
 }
 
@@ -2809,7 +2815,8 @@ int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* b, i
   const int rc = check_paged(nullptr, kv, b);
   if (rc) return rc;
   PagedAttnParams P;
-  return plan_attn(nullptr, kv, b, n_heads, window, &P, bytes);
+  int64_t parts;
+  return plan_attn(nullptr, kv, b, n_heads, window, &P, bytes, &parts);
 }
 
 int c2h_paged_attn_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int32_t type, int32_t n_heads,
@@ -2820,7 +2827,8 @@ int c2h_paged_attn_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch
   PagedAttnParams P;
   memset(&P, 0, sizeof(P));
   size_t bytes = 0;
-  if ((rc = plan_attn(c, kv, b, n_heads, window, &P, &bytes)) ||
+  int64_t parts = 0;
+  if ((rc = plan_attn(c, kv, b, n_heads, window, &P, &bytes, &parts)) ||
       (rc = check_heads(c, "q", q, type, b->n_seqs, n_heads, kv->head_dim, false)) ||
       (rc = check_heads(c, "out", out, type, b->n_seqs, n_heads, kv->head_dim, true)))
     return rc;
@@ -2828,7 +2836,7 @@ int c2h_paged_attn_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch
   if (!c) return fail(c, C2H_ERR_INVALID, "no context");
   if (b->n_seqs == 0) return C2H_OK;
   HIPCHK(c, hipSetDevice(c->device));
-  if (bytes > c->paged_ws_bytes) {
+  if (bytes > c->paged_ws_bytes) {  // a larger one, once the stream's work is done with the old
     HIPCHK(c, hipStreamSynchronize(c->stream));
     if (c->paged_ws) (void)hipFree(c->paged_ws);
     c->paged_ws = nullptr;
@@ -2844,8 +2852,11 @@ int c2h_paged_attn_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch
   P.out = head_rows(out, type);
   P.type = type;
   P.scale_log2 = (float)((double)scale * 1.44269504088896340736);
-  P.part_o = c->paged_ws;
-  P.part_ml = c->paged_ws ? c->paged_ws + (size_t)b->n_seqs * n_heads * P.n_chunks * kv->head_dim : nullptr;
+  if (parts) {
+    P.part_o = c->paged_ws;
+    P.part_ml = P.part_o + parts * kv->head_dim;
+    P.info = reinterpret_cast<int32_t*>(P.part_ml + parts * 2);
+  }
   P.err = c->tok_host + 3;
   launch_paged_attn(P, kv->type, c->stream);
   HIPCHK(c, hipGetLastError());

@@ -20,9 +20,10 @@ enum PagedErr : int { PERR_LENGTH = 1, PERR_PAGE = 2, PERR_START = 4 };
 
 constexpr int PAGED_MIN_PAGE = 8;      // a lane's four rows of V lie in one page
 constexpr int PAGED_MAX_PAGE = 1024;
+constexpr int PAGED_MAX_LEN = 1 << 23; // chunks are a grid's third index
 constexpr int ATTN_HEADS = 16;         // query heads of a workgroup: columns of the matrix instruction
-constexpr int ATTN_MAX_CHUNK = 1024;   // positions of a workgroup
-constexpr int ATTN_TAB = ATTN_MAX_CHUNK / PAGED_MIN_PAGE + 1;  // pages a chunk can touch
+constexpr int ATTN_CHUNKS = 1024;      // chunks that a batch is cut into
+constexpr int ATTN_WGS = 512;          // workgroups that take them in turn
 
 // The positions [lo, hi) that a session of `len` positions attends, `window`
 // of them at most (0: all).
@@ -32,25 +33,41 @@ struct Span {
 C2H_HD inline Span attended(int len, int window) {
   return Span{window > 0 && len > window ? len - window : 0, len};
 }
-// The span's chunks begin at multiples of `chunk` from its first position
-// rounded down to a multiple of 4, so that four positions a lane reads
-// together lie in one page; the first chunk's begin at s.lo.
+// A span is cut into chunks of whole units, of the positions that the four
+// waves of a workgroup take in one step.  Chunks begin at multiples of their
+// size from the span's first position rounded down to a multiple of 4, so that
+// four positions a lane reads together lie in one page; the first chunk's
+// begin at s.lo.
 constexpr int SPAN_ALIGN = 4;
 C2H_HD inline int chunk_base(Span s, int chunk, int i) { return (s.lo & ~(SPAN_ALIGN - 1)) + i * chunk; }
-C2H_HD inline int chunks_of(Span s, int chunk) {
-  return (int)(((int64_t)s.hi - (s.lo & ~(SPAN_ALIGN - 1)) + chunk - 1) / chunk);
+C2H_HD inline int units_of(Span s, int unit) { return (s.hi - (s.lo & ~(SPAN_ALIGN - 1)) + unit - 1) / unit; }
+// Chunks of a session: at least one, which writes the row of an empty one.
+C2H_HD inline int chunks_of(int units, int chunk_units) {
+  const int n = (units + chunk_units - 1) / chunk_units;
+  return n > 1 ? n : 1;
 }
-// Chunks of the longest span of a launch: sessions of at most max_len.
-C2H_HD inline int most_chunks(int max_len, int window, int chunk) {
-  return window > 0 && window < max_len ? chunks_of(Span{0, window + SPAN_ALIGN - 1}, chunk) : chunks_of(Span{0, max_len}, chunk);
+// Tiles of 16 positions in a wave's step: 16 KB of keys and values, at most
+// four tiles and at least one.
+C2H_HD constexpr int attn_tiles(int type, int hd) {
+  const int t = 512 / (hd * type_bytes(type));
+  return t < 1 ? 1 : t > 4 ? 4 : t;
 }
-
-// Positions per workgroup for a batch of n_rows (session, KV head, head
-// tile) rows whose spans are at most `span`.
-inline int attn_chunk(int64_t n_rows, int span) {
-  int chunk = ATTN_MAX_CHUNK;
-  while (chunk > 128 && n_rows * ((span + chunk - 1) / chunk) < 1024) chunk /= 2;
-  return chunk;
+C2H_HD constexpr int attn_hd(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+C2H_HD constexpr int attn_unit(int type, int head_dim) { return 64 * attn_tiles(type, attn_hd(head_dim)); }
+// Units of a chunk whose pages a wave's lanes hold, one each.
+C2H_HD constexpr int most_units(int unit, int page_size) { return (64 - 1) * page_size / unit; }
+// Units per chunk: a batch of `units` in all, in each of n_rows (KV head, head
+// tile) rows, as about ATTN_CHUNKS equal chunks.
+C2H_HD inline int chunk_units(int64_t units, int n_rows, int most) {
+  const int64_t c = (units * n_rows + ATTN_CHUNKS - 1) / ATTN_CHUNKS;
+  return (int)(c < 1 ? 1 : c > most ? most : c);
+}
+// Chunks (of one row) that any batch can come to: about ATTN_CHUNKS / n_rows, and a
+// partial one per session, unless `most` cuts them shorter.
+inline int64_t chunks_bound(int n_seqs, int n_rows, int max_units, int most) {
+  const int64_t even = ATTN_CHUNKS / n_rows + 1 + n_seqs, cut = (int64_t)n_seqs * chunks_of(max_units, most);
+  const int64_t all = (int64_t)n_seqs * (max_units > 1 ? max_units : 1), b = even > cut ? even : cut;
+  return b < all ? b : all;
 }
 
 C2H_HD inline bool length_ok(int len, int max_len) { return len >= 0 && len <= max_len; }
@@ -87,10 +104,13 @@ struct PagedAttnParams {
   int type;        // of q and out
   int n_heads, group, n_tiles;  // query heads, per KV head, workgroups of ATTN_HEADS of them
   int window;
-  int chunk, n_chunks;          // positions per workgroup; chunks of the longest session
+  int n_rows;                   // n_kv_heads * n_tiles
+  int most;                     // units of a chunk at most
+  int grid;                     // workgroups
   float scale_log2;             // scale * log2(e)
-  float* part_o;   // [n_seqs][n_heads][n_chunks][head_dim], where n_chunks > 1
-  float* part_ml;  // [n_seqs][n_heads][n_chunks][2]: running maximum (log2) and sum
+  float* part_o;   // [chunks_bound][n_heads][head_dim]: sums of a chunk
+  float* part_ml;  // [chunks_bound][n_heads][2]: its maximum (log2) and total
+  int32_t* info;   // [n_seqs][2]: a session's first chunk, and its chunks (null: one each)
   int* err;
 };
 

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 
+#include "c2h_device.h"
 #include "c2h_paged.h"
 
 namespace c2h {
@@ -390,10 +391,8 @@ struct Attn {
   static constexpr int VW = VB / 4, VE = VB / ES;      // its dwords, its elements
   static constexpr int NV = HD * ES / 16 / VB;         // loads of a value per lane
   static constexpr int NO = HD / 16;                   // output tiles: NV * VE
-  // tiles of 16 positions per step: 16 KB of keys and values per wave (f32
-  // of 256: 32 KB)
-  static constexpr int NT = 256 / (HD * ES) < 1 ? 1 : 512 / (HD * ES) < 1 ? 1 : 512 / (HD * ES);
-  static constexpr int STEP = 16 * NT;
+  static constexpr int NT = attn_tiles(CT, HD), STEP = 16 * NT, UNIT = 4 * STEP;
+  static_assert(UNIT == attn_unit(CT, HD), "the host's units");
   static constexpr int NQ = F32 ? 1 : PRECISE ? (BF ? 3 : 2) : 1;
   static constexpr int NP = F32 ? 1 : BF && PRECISE ? 3 : 2;
   static constexpr int FR = F32 ? HD / 16 : HD / 32;   // 16-byte fragments of a query per lane
@@ -404,48 +403,208 @@ struct Attn {
   static constexpr int LDS = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
 };
 
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int scan_of_wave(int x) {
+  x += dpp0_i<0x111>(x);  // row_shr:1
+  x += dpp0_i<0x112>(x);
+  x += dpp0_i<0x114>(x);
+  x += dpp0_i<0x118>(x);
+  x += dpp0_i<DPP_BCAST15, 0xa>(x);
+  x += dpp0_i<DPP_BCAST31, 0xc>(x);
+  return x;
+}
+
+// How a batch is cut, found by every wave from the lengths: the host does not
+// know them, and a grid over max_len would start a workgroup per chunk that a
+// session could have (64 sessions of 30 to 8,000: most of them empty).  Lane l
+// looks after sessions [l * per, (l + 1) * per).
+struct Cut {
+  int per, units;   // units: positions of a chunk, in units
+  int len;          // per == 1: the lane's length
+  int upto;         // chunks of the sessions up to this lane's last
+  int total;
+};
+template <int UNIT>
+__device__ __forceinline__ int session_units(int len, int max_len, int window) {
+  return units_of(attended(length_ok(len, max_len) ? len : 0, window), UNIT);
+}
+template <int UNIT>
+__device__ __forceinline__ Cut cut_batch(const int32_t* lens, int n_seqs, int max_len, int window, int n_rows, int most,
+                                         bool split) {
+  const int lane = threadIdx.x & 63;
+  Cut c{(n_seqs + 63) >> 6, 1, 0, 0, n_seqs};
+  if (!split) return c;  // no session is longer than a unit
+  int64_t units = 0;
+  if (c.per == 1) {
+    c.len = lane < n_seqs ? lens[lane] : 0;
+    units = __builtin_amdgcn_readlane(scan_of_wave(session_units<UNIT>(c.len, max_len, window)), 63);
+  } else {
+    int mine = 0;  // below 2^31: 1024 sessions of 2^17 units
+    for (int k = 0; k < c.per; ++k) {
+      const int s = lane * c.per + k;
+      mine += s < n_seqs ? session_units<UNIT>(lens[s], max_len, window) : 0;
+    }
+    for (int m = 0; m < 64; ++m) units += __builtin_amdgcn_readlane(mine, m);
+  }
+  c.units = chunk_units(units, n_rows, most);
+  int n = 0;
+  if (c.per == 1) {
+    n = lane < n_seqs ? chunks_of(session_units<UNIT>(c.len, max_len, window), c.units) : 0;
+  } else {
+    for (int k = 0; k < c.per; ++k) {
+      const int s = lane * c.per + k;
+      n += s < n_seqs ? chunks_of(session_units<UNIT>(lens[s], max_len, window), c.units) : 0;
+    }
+  }
+  c.upto = scan_of_wave(n);
+  c.total = __builtin_amdgcn_readlane(c.upto, 63);
+  return c;
+}
+
+// The leading arguments arrive in registers at wave start (kernel-argument
+// preload).  shape: log2 of the page size; bit 8: sessions can have several
+// chunks; n_tiles from bit 16.
 template <int CT, int HD, bool FULL, bool PRECISE>
-__global__ void __launch_bounds__(256, (CT == PT_F32 && HD == 256) ? 1 : 2) k_paged_attn(PagedAttnParams P) {
+__global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 : 2)
+    k_paged_attn(const int32_t* lens, const int32_t* table, int64_t table_stride, int max_len, int window, uint32_t shape,
+                 int n_seqs, PagedAttnParams P) {
   using A = Attn<CT, HD, FULL, PRECISE>;
   constexpr int KC = A::KC, NT = A::NT, NV = A::NV, VW = A::VW, VE = A::VE, NO = A::NO, FR = A::FR, NQ = A::NQ, NP = A::NP;
   constexpr bool BF = A::BF;
   __shared__ __align__(16) char lds[A::LDS];
-  __shared__ int64_t tab[ATTN_TAB];  // the pages' offsets in the pool
-  __shared__ int bad;
   __shared__ float mul[16], wm[4][16], wl[4][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, j = lane >> 4;
-  const int chunk = blockIdx.x, s = blockIdx.z;
-  const int kvh = blockIdx.y / P.n_tiles, h0 = kvh * P.group + (blockIdx.y - kvh * P.n_tiles) * ATTN_HEADS;
-  const int nh = min(ATTN_HEADS, (kvh + 1) * P.group - h0);
-  const int hd = FULL ? HD : P.kv.head_dim, shift = P.kv.page_shift;
+  const int shift = shape & 255, n_tiles = shape >> 16;
+  const bool split = shape & 256;
+  const Cut cut = cut_batch<A::UNIT>(lens, n_seqs, max_len, window, P.n_rows, P.most, split);
+  const int csize = cut.units * A::UNIT, items = cut.total * P.n_rows;
 
-  const int len = P.b.lens[s];
-  const bool ok = length_ok(len, P.b.max_len);
-  const Span span = attended(ok ? len : 0, P.window);
-  const int n = max(chunks_of(span, P.chunk), 1);
-  if (chunk >= n) return;
-  const int base0 = chunk_base(span, P.chunk, chunk), c0 = max(base0, span.lo), c1 = min(base0 + P.chunk, span.hi);
-  const int p0 = c0 >> shift;
-
-  // the chunk's pages, and the queries split into the parts of the product
-  if (tid == 0) bad = !ok;
-  __syncthreads();
-  for (int i = tid; i <= ((c1 - 1) >> shift) - p0 && c1 > c0; i += 256) {
-    const int page = P.b.table[s * P.b.table_stride + p0 + i];
-    tab[i] = page * P.kv.page_stride + kvh * P.kv.head_stride;
-    if (!page_ok(page, P.kv.n_pages)) bad = 2;
-  }
-  {
-    constexpr int EPT = HD / 16;  // elements per thread
-    const int head = tid >> 4, d0 = (tid & 15) * EPT;
-    f32x4 q[EPT / 4];
-#pragma unroll
-    for (int g = 0; g < EPT / 4; ++g) {
-      const bool have = head < nh && (FULL || d0 + 4 * g < hd);
-      q[g] = have ? load4(P.type, P.q.data + s * P.q.token_stride + (h0 + head) * P.q.head_stride +
-                                      (int64_t)(d0 + 4 * g) * (P.type == PT_F32 ? 4 : 2))
-                  : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+  // the item's session and chunk
+  const int unit = item / P.n_rows, row = item - unit * P.n_rows;
+  int s = unit, chunk = 0, len = 0;
+  if (!split) {
+    len = lens[s];
+  } else {
+    const int owner = __popcll(__ballot(cut.upto <= unit));
+    chunk = unit - (owner ? __builtin_amdgcn_readlane(cut.upto, owner - 1) : 0);
+    s = owner;
+    len = __builtin_amdgcn_readlane(cut.len, owner);
+    if (cut.per > 1) {
+      len = 0;
+      for (s = owner * cut.per; s < min((owner + 1) * cut.per, n_seqs); s += 64) {  // 64 at a time; one of them has it
+        const bool mine = s + lane < n_seqs && s + lane < (owner + 1) * cut.per;
+        const int one = mine ? lens[s + lane] : 0;
+        const int upto = scan_of_wave(mine ? chunks_of(session_units<A::UNIT>(one, max_len, window), cut.units) : 0);
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        if (chunk < all) {
+          const int at = __popcll(__ballot(upto <= chunk));
+          chunk -= at ? __builtin_amdgcn_readlane(upto, at - 1) : 0;
+          len = __builtin_amdgcn_readlane(one, at);
+          s += at;
+          break;
+        }
+        chunk -= all;
+      }
+      s = min(s, n_seqs - 1);
     }
+  }
+  const bool ok = length_ok(len, max_len);
+  const Span span = attended(ok ? len : 0, window);
+  const int n = chunks_of(units_of(span, A::UNIT), cut.units);
+  const int base0 = chunk_base(span, csize, chunk), c0 = max(base0, span.lo), c1 = min(base0 + csize, span.hi);
+  const int p0 = c0 >> shift, last = c1 - 1;
+  if (split && row == 0 && chunk == 0 && tid == 0) {
+    P.info[2 * s] = unit;
+    P.info[2 * s + 1] = n;
+  }
+  // lane i holds page p0 + i: a chunk has at most 64
+  const bool paged = lane <= (last >> shift) - p0 && c1 > c0;
+  const int page = paged ? table[s * table_stride + p0 + lane] : 0;
+
+  const int kvh = n_tiles == 1 ? row : row / n_tiles;
+  const int h0 = kvh * P.group + (row - kvh * n_tiles) * ATTN_HEADS;
+  const int nh = min(ATTN_HEADS, (kvh + 1) * P.group - h0);
+  const int hd = FULL ? HD : P.kv.head_dim;
+  constexpr int EPT = HD / 16;  // elements of the queries that a thread brings
+  const int qhead = tid >> 4, qd0 = (tid & 15) * EPT;
+  f32x4 q[EPT / 4];
+#pragma unroll
+  for (int g = 0; g < EPT / 4; ++g) {
+    const bool have = qhead < nh && (FULL || qd0 + 4 * g < hd);
+    q[g] = have ? load4(P.type, P.q.data + s * P.q.token_stride + (h0 + qhead) * P.q.head_stride +
+                                    (int64_t)(qd0 + 4 * g) * (P.type == PT_F32 ? 4 : 2))
+                : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  const bool fail = !ok || __any(paged && !page_ok(page, P.kv.n_pages));
+  const int64_t page_off = page * P.kv.page_stride + kvh * P.kv.head_stride;
+
+  u32x4 K[NT][KC];
+  uint32_t V[NT][4][NV][VW];
+  const int rowb = hd * A::ES, mask = (1 << shift) - 1;
+  const uint32_t ts = (uint32_t)P.kv.token_stride;  // below 2^31
+  // Positions outside [c0, c1) are read as the nearest inside, and masked
+  // in the scores; elements past head_dim as the row's first, against zeros
+  // of Q and into output tiles that are not stored.
+  auto inside = [&](int pos) { return min(max(pos, c0), last); };
+  auto page_of = [&](int pos) {
+    const int at = ((pos >> shift) - p0) * 4;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)page_off);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)(page_off >> 32));
+    return (int64_t)((uint64_t)hi << 32 | lo);
+  };
+  auto in_page = [&](int pos) { return (int64_t)((uint64_t)(uint32_t)(pos & mask) * ts); };
+  auto load_k = [&](int base) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int pos = inside(base + 16 * t + r);
+      const char* row = P.kv.k + page_of(pos) + in_page(pos);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        int off = c * 64 + j * 16;
+        if constexpr (!FULL) off = off < rowb ? off : 0;
+        K[t][c] = *reinterpret_cast<const u32x4*>(row + off);
+      }
+    }
+  };
+  auto load_v = [&](int base) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      // one page holds those of the four positions that are inside
+      const int first = base + 16 * t + 4 * j;
+      const char* at = P.kv.v + page_of(inside(first));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const char* row = at + in_page(inside(first + i));
+#pragma unroll
+        for (int b = 0; b < NV; ++b) {
+          int off = b * 16 * A::VB + r * A::VB;
+          if constexpr (!FULL) off = off < rowb ? off : 0;
+          if constexpr (VW == 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(row + off);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) V[t][i][b][w] = v[w];
+          } else if constexpr (VW == 2) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(row + off);
+            V[t][i][b][0] = v.x;
+            V[t][i][b][1] = v.y;
+          } else {
+            V[t][i][b][0] = *reinterpret_cast<const uint32_t*>(row + off);
+          }
+        }
+      }
+    }
+  };
+  const bool work = !fail && base0 + wave * A::STEP < c1;
+  if (work) {
+    load_k(base0 + wave * A::STEP);
+    load_v(base0 + wave * A::STEP);
+  }
+
+  // the queries, split into the parts of the product
+  __syncthreads();  // the item before is done with LDS
+  {
     int e = 0;
     if constexpr (A::BIAS != 0.0f) {
       float top = 0.0f;
@@ -461,16 +620,16 @@ __global__ void __launch_bounds__(256, (CT == PT_F32 && HD == 256) ? 1 : 2) k_pa
     }
     if ((tid & 15) == 0) {
       const float ks = A::F8 && P.kv.k_scale ? P.kv.k_scale[kvh] : 1.0f;
-      mul[head] = ldexpf(P.scale_log2 * ks, -e);
+      mul[qhead] = ldexpf(P.scale_log2 * ks, -e);
     }
 #pragma unroll
     for (int g = 0; g < EPT / 4; ++g) {
-      const int d = d0 + 4 * g;
+      const int d = qd0 + 4 * g;
       if constexpr (A::F32) {
-        *reinterpret_cast<f32x4*>(lds + ((d >> 4) * 64 + ((d >> 2) & 3) * 16 + head) * 16) = q[g];
+        *reinterpret_cast<f32x4*>(lds + ((d >> 4) * 64 + ((d >> 2) & 3) * 16 + qhead) * 16) = q[g];
       } else {
         const int f = A::F8 ? 2 * (d >> 6) + ((d >> 3) & 1) : d >> 5, jj = A::F8 ? (d >> 4) & 3 : (d >> 3) & 3;
-        char* at = lds + (f * 64 + jj * 16 + head) * 16 + ((d >> 2) & 1) * 8;
+        char* at = lds + (f * 64 + jj * 16 + qhead) * 16 + ((d >> 2) & 1) * 8;
         float a[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = A::BIAS != 0.0f ? ldexpf(q[g][i], e) : q[g][i];
@@ -482,7 +641,6 @@ __global__ void __launch_bounds__(256, (CT == PT_F32 && HD == 256) ? 1 : 2) k_pa
     }
   }
   __syncthreads();
-  const bool fail = bad != 0;
   const float smul = mul[r];
 
   f32x4 o[NO];
@@ -490,60 +648,7 @@ __global__ void __launch_bounds__(256, (CT == PT_F32 && HD == 256) ? 1 : 2) k_pa
   for (int t = 0; t < NO; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   float m = MINUS_INF, l = 0.0f;
 
-  if (!fail && base0 + wave * A::STEP < c1) {
-    u32x4 K[NT][KC];
-    uint32_t V[NT][4][NV][VW];
-    const int rowb = hd * A::ES, mask = (1 << shift) - 1, last = c1 - 1;
-    const uint32_t ts = (uint32_t)P.kv.token_stride;  // below 2^31
-    // Positions outside [c0, c1) are read as the nearest inside, and masked
-    // in the scores; elements past head_dim as the row's first, against zeros
-    // of Q and into output tiles that are not stored.
-    auto inside = [&](int pos) { return min(max(pos, c0), last); };
-    auto page_of = [&](int pos) { return tab[(pos >> shift) - p0]; };
-    auto in_page = [&](int pos) { return (int64_t)((uint64_t)(uint32_t)(pos & mask) * ts); };
-    auto load_k = [&](int base) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int pos = inside(base + 16 * t + r);
-        const char* row = P.kv.k + page_of(pos) + in_page(pos);
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          int off = c * 64 + j * 16;
-          if constexpr (!FULL) off = off < rowb ? off : 0;
-          K[t][c] = *reinterpret_cast<const u32x4*>(row + off);
-        }
-      }
-    };
-    auto load_v = [&](int base) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        // one page holds those of the four positions that are inside
-        const int first = base + 16 * t + 4 * j;
-        const char* page = P.kv.v + page_of(inside(first));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const char* row = page + in_page(inside(first + i));
-#pragma unroll
-          for (int b = 0; b < NV; ++b) {
-            int off = b * 16 * A::VB + r * A::VB;
-            if constexpr (!FULL) off = off < rowb ? off : 0;
-            if constexpr (VW == 4) {
-              const u32x4 v = *reinterpret_cast<const u32x4*>(row + off);
-#pragma unroll
-              for (int w = 0; w < 4; ++w) V[t][i][b][w] = v[w];
-            } else if constexpr (VW == 2) {
-              const u32x2 v = *reinterpret_cast<const u32x2*>(row + off);
-              V[t][i][b][0] = v.x;
-              V[t][i][b][1] = v.y;
-            } else {
-              V[t][i][b][0] = *reinterpret_cast<const uint32_t*>(row + off);
-            }
-          }
-        }
-      }
-    };
-    load_k(base0 + wave * A::STEP);
-    load_v(base0 + wave * A::STEP);
+  if (work) {
     for (int base = base0 + wave * A::STEP; base < c1; base += 4 * A::STEP) {
       const int next = base + 4 * A::STEP;
       // scores
@@ -694,50 +799,68 @@ __global__ void __launch_bounds__(256, (CT == PT_F32 && HD == 256) ? 1 : 2) k_pa
         sum += *reinterpret_cast<const f32x4*>(os + (w * 16 + head) * A::OROW + d) * a;
       }
       if (fail) sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f} + __builtin_nanf("");
-      const int64_t row = (int64_t)s * P.n_heads + h0 + head;
       if (n == 1) {
         const float inv = fail ? 1.0f : total == 0.0f ? 0.0f : vs / total;
         store4(P.type, P.out.data + s * P.out.token_stride + (h0 + head) * P.out.head_stride +
                            (int64_t)(d0 + d) * (P.type == PT_F32 ? 4 : 2), sum * inv);
       } else {
-        *reinterpret_cast<f32x4*>(P.part_o + (row * P.n_chunks + chunk) * hd + d0 + d) = sum * vs;
+        const int64_t part = (int64_t)unit * P.n_heads + h0 + head;
+        *reinterpret_cast<f32x4*>(P.part_o + part * hd + d0 + d) = sum * vs;
         if (d0 + d == 0) {
-          P.part_ml[(row * P.n_chunks + chunk) * 2] = top;
-          P.part_ml[(row * P.n_chunks + chunk) * 2 + 1] = total;
+          P.part_ml[part * 2] = top;
+          P.part_ml[part * 2 + 1] = total;
         }
       }
     }
   }
   if (fail && tid == 0) report(P.err, ok ? PERR_PAGE : PERR_LENGTH);
+  }
 }
 
 // Joins the chunks of a row: the sums brought to the common maximum.  One
-// workgroup per row; HDP / 4 threads hold the row's elements, 1024 / HDP
-// groups of them every so-manieth chunk each.
+// workgroup per row; HDP / 4 threads hold the row's elements, and 1024 / HDP
+// groups of them take every so-manieth chunk.
 template <int HDP>
-__global__ void __launch_bounds__(256) k_paged_join(PagedAttnParams P) {
-  constexpr int LANES = HDP / 4, GROUPS = 256 / LANES;
-  __shared__ float tmp[4];
+__global__ void __launch_bounds__(256) k_paged_join(const int32_t* info, const float* part_o, const float* part_ml,
+                                                    PagedAttnParams P) {
+  constexpr int LANES = HDP / 4, GROUPS = 256 / LANES, AHEAD = 4;
   __shared__ __align__(16) float part[GROUPS][HDP + 4];
+  __shared__ float tmp[4];
   const int head = blockIdx.x, s = blockIdx.y, hd = P.kv.head_dim, tid = threadIdx.x;
-  const int len = P.b.lens[s];
-  const int n = chunks_of(attended(length_ok(len, P.b.max_len) ? len : 0, P.window), P.chunk);
+  const int g = tid / LANES, d = (tid % LANES) * 4, dc = min(d, hd - 4);
+  const int n = info[2 * s + 1];
   if (n <= 1) return;
-  const int64_t row = ((int64_t)s * P.n_heads + head) * P.n_chunks;
-  const float2* ml = reinterpret_cast<const float2*>(P.part_ml) + row;
+  const int64_t first = (int64_t)info[2 * s] * P.n_heads + head;
+  auto ml = [&](int i) { return *reinterpret_cast<const float2*>(part_ml + (first + (int64_t)i * P.n_heads) * 2); };
+  auto sums = [&](int i) { return *reinterpret_cast<const f32x4*>(part_o + (first + (int64_t)i * P.n_heads) * hd + dc); };
+  float2 x[AHEAD];
+  f32x4 v[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = min(g + k * GROUPS, n - 1);
+    x[k] = ml(i);
+    v[k] = sums(i);
+  }
   float m = MINUS_INF;
-  for (int i = tid; i < n; i += 256) m = fmaxf(m, ml[i].x);
+  for (int i = tid; i < n; i += 256) m = fmaxf(m, ml(i).x);
   for (int k = 32; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
   if ((tid & 63) == 0) tmp[tid >> 6] = m;
   __syncthreads();
   const float mu = finite_max(fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3])));
-  const int g = tid / LANES, d = (tid % LANES) * 4;
   f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
   float l = 0.0f;
-  for (int i = g; i < n; i += GROUPS) {
-    const float w = weight(ml[i].x, mu);
-    l += ml[i].y * w;
-    if (d < hd) a += *reinterpret_cast<const f32x4*>(P.part_o + (row + i) * hd + d) * w;
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (g + k * GROUPS < n) {
+      const float w = weight(x[k].x, mu);
+      l += x[k].y * w;
+      a += v[k] * w;
+    }
+  for (int i = g + AHEAD * GROUPS; i < n; i += GROUPS) {
+    const float2 y = ml(i);
+    const float w = weight(y.x, mu);
+    l += y.y * w;
+    a += sums(i) * w;
   }
   *reinterpret_cast<f32x4*>(&part[g][d]) = a;
   if (d == 0) part[g][HDP] = l;
@@ -758,9 +881,11 @@ __global__ void __launch_bounds__(256) k_paged_join(PagedAttnParams P) {
 
 template <int CT, int HD, bool FULL, bool PRECISE>
 void launch_attn_as(const PagedAttnParams& P, hipStream_t st) {
-  const dim3 grid(P.n_chunks, P.kv.n_kv_heads * P.n_tiles, P.b.n_seqs);
-  hipLaunchKernelGGL((k_paged_attn<CT, HD, FULL, PRECISE>), grid, dim3(256), 0, st, P);
-  if (P.n_chunks > 1) hipLaunchKernelGGL(k_paged_join<HD>, dim3(P.n_heads, P.b.n_seqs), dim3(256), 0, st, P);
+  const uint32_t shape = (uint32_t)P.kv.page_shift | (P.info ? 256u : 0u) | (uint32_t)P.n_tiles << 16;
+  hipLaunchKernelGGL((k_paged_attn<CT, HD, FULL, PRECISE>), dim3(P.grid), dim3(256), 0, st, P.b.lens, P.b.table,
+                     P.b.table_stride, P.b.max_len, P.window, shape, P.b.n_seqs, P);
+  if (P.info)
+    hipLaunchKernelGGL(k_paged_join<HD>, dim3(P.n_heads, P.b.n_seqs), dim3(256), 0, st, P.info, P.part_o, P.part_ml, P);
 }
 
 // Queries and outputs that a single 16-bit part holds take the shorter

@@ -52,7 +52,7 @@ BAD_CACHE = [
     (dict(page_stride=1 << 50), INVALID, "strides"),
 ]
 BAD_BATCH = [
-    (dict(n_seqs=-1), "sessions"), (dict(max_len=-1), "max_len"), (dict(max_len=(1 << 30) + 1), "max_len"),
+    (dict(n_seqs=-1), "sessions"), (dict(max_len=-1), "max_len"), (dict(max_len=(1 << 23) + 1, table_stride=1 << 30), "max_len"),
     (dict(block_table=None), "table"), (dict(seq_lens=None), "lengths"), (dict(max_len=129), "does not cover"),
     (dict(table_stride=-1), "does not cover"),
 ]
@@ -162,12 +162,11 @@ def test_norm_arguments_refused():
 
 
 def test_workspace_follows_the_split():
-    # a batch that fills the GPU with whole sessions needs none; one long
-    # session is split, and its parts are head_dim + 2 floats per query head
-    assert H.paged_attn_workspace(kv(n_kv_heads=8, page_stride=16 * 512, token_stride=512),
-                                  batch(n_seqs=512, max_len=100), 16) == 0
+    # sessions that one step of a workgroup holds need none; longer ones meet
+    # in head_dim + 2 floats per query head and chunk, and two integers each
     one = batch(n_seqs=1, max_len=8192, table_stride=512)
-    got = H.paged_attn_workspace(kv(), one, 14)
+    assert H.paged_attn_workspace(kv(), batch(n_seqs=512, max_len=100), 14) == 0
+    got = H.paged_attn_workspace(kv(), one, 14) - 8
     assert got > 0 and got % (14 * (64 + 2) * 4) == 0
     # a window bounds it
     assert H.paged_attn_workspace(kv(), one, 14, window=100) == 0
@@ -224,35 +223,49 @@ int main() {
   assert(page_ok(0, 1) && page_ok(99, 100) && !page_ok(100, 100) && !page_ok(-1, 100) && !page_ok(INT_MIN, 100) &&
          !page_ok(INT_MAX, 100));
   assert(length_ok(0, 0) && length_ok(5, 5) && !length_ok(6, 5) && !length_ok(-1, 5) && !length_ok(INT_MIN, 1 << 30));
-  // windows and chunks cover the span once, in order, without overflow
-  const int lens[] = {0, 1, 2, 127, 128, 129, 4095, 4096, 100001, 1 << 30};
+  // windows and chunks cover the span once, in order, without overflow, and
+  // a chunk's pages are at most a wave's lanes
+  const int lens[] = {0, 1, 2, 127, 128, 129, 4095, 4096, 100001, PAGED_MAX_LEN};
   const int wins[] = {0, 1, 127, 128, 1000, 1 << 30};
   for (int len : lens)
     for (int w : wins)
-      for (int chunk : {128, 256, 1024}) {
-        const Span s = attended(len, w);
-        assert(s.hi == len && s.lo >= 0 && s.hi - s.lo == (w > 0 && w < len ? w : len));
-        const int n = chunks_of(s, chunk);
-        assert(len == 0 ? n == 0 : n >= 1 && n <= most_chunks(len, w, chunk) && n <= most_chunks(1 << 30, w, chunk));
-        int64_t at = s.lo;
-        for (int i = 0; i < n; i = i == 2 && n > 6 ? n - 3 : i + 1) {  // the first and last three
-          const int64_t b = chunk_base(s, chunk, i), c0 = b > s.lo ? b : s.lo, c1 = b + chunk < s.hi ? b + chunk : s.hi;
-          assert(b % SPAN_ALIGN == 0 && c1 > c0 && c1 - c0 <= chunk && (i < 3 ? c0 == at : c0 > s.lo));
-          at = c1;
-          // the pages that a chunk touches fit its table
-          for (int sh = 3; sh <= 10; ++sh) assert(((c1 - 1) >> sh) - (c0 >> sh) + 1 <= ATTN_TAB);
+      for (int unit : {64, 128, 256})
+        for (int page = 8; page <= 1024; page *= 2)
+          for (int cu : {1, 2, 3, 7, most_units(unit, page)}) {
+            if (cu > most_units(unit, page)) continue;
+            const int chunk = cu * unit;
+            const Span s = attended(len, w);
+            assert(s.hi == len && s.lo >= 0 && s.hi - s.lo == (w > 0 && w < len ? w : len));
+            const int units = units_of(s, unit), n = chunks_of(units, cu);
+            const int longest = w > 0 && w < PAGED_MAX_LEN ? w + SPAN_ALIGN - 1 : PAGED_MAX_LEN;
+            assert(n >= 1 && (units == 0) == (len == 0) && units <= units_of(Span{0, longest}, unit));
+            int64_t at = s.lo;
+            for (int i = 0; len > 0 && i < n; i = i == 2 && n > 6 ? n - 3 : i + 1) {  // the first and last three
+              const int64_t b = chunk_base(s, chunk, i), c0 = b > s.lo ? b : s.lo, c1 = b + chunk < s.hi ? b + chunk : s.hi;
+              assert(b % SPAN_ALIGN == 0 && c1 > c0 && c1 - c0 <= chunk && (i < 3 ? c0 == at : c0 > s.lo));
+              at = c1;
+              assert((c1 - 1) / page - c0 / page < 64);
+            }
+            assert(at == s.hi);
+          }
+  // the bound of a batch's chunks holds for even and uneven batches
+  for (int n_seqs : {1, 2, 63, 64, 65, 700})
+    for (int rows : {1, 2, 8, 600})
+      for (int most : {1, 4, 30})
+        for (int shape = 0; shape < 4; ++shape) {
+          int64_t units = 0, chunks = 0;
+          auto u = [&](int i) { return shape == 0 ? 0 : shape == 1 ? 50 : shape == 2 ? (i * 7919) % 51 : i ? 1 : 50; };
+          for (int i = 0; i < n_seqs; ++i) units += u(i);
+          const int cu = chunk_units(units, rows, most);
+          assert(cu >= 1 && cu <= most);
+          for (int i = 0; i < n_seqs; ++i) chunks += chunks_of(u(i), cu);
+          assert(chunks <= chunks_bound(n_seqs, rows, 50, most));
         }
-        assert(at == s.hi);
-      }
+  for (int type : {PT_F32, PT_F16, PT_BF16, PT_E4M3})
+    for (int hd = 16; hd <= 256; hd += 16) assert(most_units(attn_unit(type, hd), PAGED_MIN_PAGE) >= 1);
   // the tokens of a session are its last ones
   assert(token_pos(10, 5, 6) == 9 && token_pos(10, 0, 6) == 4 && token_pos(3, 0, 6) == -3 && token_pos(0, 0, 1) == -1);
   assert(token_pos(1 << 30, INT_MAX - 1, INT_MAX) == (1 << 30) - 1);
-  // the split: whole chunks, never beyond what a workgroup holds
-  for (int64_t rows : {(int64_t)1, (int64_t)2, (int64_t)14, (int64_t)1000, (int64_t)1 << 24})
-    for (int span : {0, 1, 128, 5000, 1 << 30}) {
-      const int c = attn_chunk(rows, span);
-      assert(c >= 128 && c <= ATTN_MAX_CHUNK && c % 128 == 0);
-    }
   puts("ok");
 }
 """
