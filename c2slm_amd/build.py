@@ -45,22 +45,24 @@ def build(verbose: bool = False) -> str:
     flags = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-ffp-contract=off",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *PRELOAD,
              "-Wall", "-Wno-unused-function", "-I", os.path.join(HERE, "..", "include")]
-    objs = []
     bdir = os.path.join(HERE, "_build")
     os.makedirs(bdir, exist_ok=True)
-    for src in SOURCES:
+    jobs = []
+    for src in SOURCES:  # side by side
         path = os.path.join(CSRC, src)
         if not os.path.exists(path):
             raise FileNotFoundError(path)
         obj = os.path.join(bdir, src + ".o")
         cmd = [hipcc(), *flags, "-c", path, "-o", obj]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        if res.returncode != 0:
-            sys.stderr.write(res.stdout + res.stderr)
+        jobs.append((src, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    said = [(src, job.communicate()[0], job.returncode) for src, _, job in jobs]
+    for src, out, rc in said:
+        if rc != 0:
+            sys.stderr.write(out)
             raise RuntimeError(f"hipcc failed on {src}")
         if verbose:
-            sys.stderr.write(res.stderr)
-        objs.append(obj)
+            sys.stderr.write(out)
+    objs = [obj for _, obj, _ in jobs]
     tmp = LIB + ".tmp"
     cmd = [hipcc(), "-shared", "-fPIC", f"--offload-arch={ARCH}", *objs, "-o", tmp]
     res = subprocess.run(cmd, capture_output=True, text=True)
