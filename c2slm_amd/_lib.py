@@ -397,28 +397,38 @@ class Ctx:
     def rope_dev(self, rope: Rope, ggml_type: int, x: Heads, positions, n_tokens: int, n_heads: int, head_dim: int,
                  y: Heads):
         """y = x rotated to positions (c2h_rope_dev)."""
-        self._chk(lib().c2h_rope_dev(self.h, rope, ggml_type, x, _dp(positions), n_tokens, n_heads, head_dim, y))
+        rc = _lib.c2h_rope_dev(self.h, rope, ggml_type, x, _dp(positions), n_tokens, n_heads, head_dim, y)
+        if rc:
+            self._chk(rc)
 
     def paged_append_dev(self, kv: PagedKV, batch: PagedBatch, ggml_type: int, n_tokens: int, k: Heads, v: Heads,
                          token_start=None, rope: Rope | None = None, q: Heads | None = None, q_out: Heads | None = None,
                          n_heads: int = 0):
         """Keys and values of new tokens into their pages, K rotated, and the
         queries rotated to q_out (c2h_paged_append_dev)."""
-        self._chk(lib().c2h_paged_append_dev(self.h, kv, batch, _dp(token_start), n_tokens, rope, ggml_type, k, v,
-                                             n_heads, q, q_out))
+        rc = _lib.c2h_paged_append_dev(self.h, kv, batch, _dp(token_start), n_tokens, rope, ggml_type, k, v, n_heads, q,
+                                       q_out)
+        if rc:
+            self._chk(rc)
 
     def paged_attn_dev(self, kv: PagedKV, batch: PagedBatch, ggml_type: int, n_heads: int, scale: float, q: Heads,
                        out: Heads, window: int = 0):
         """One new token per session over its pages (c2h_paged_attn_dev)."""
-        self._chk(lib().c2h_paged_attn_dev(self.h, kv, batch, ggml_type, n_heads, scale, window, q, out))
+        rc = _lib.c2h_paged_attn_dev(self.h, kv, batch, ggml_type, n_heads, scale, window, q, out)
+        if rc:
+            self._chk(rc)
 
     def rmsnorm_q8k_dev(self, ggml_type: int, x, w, eps: float, q8k, residual=None, sum_out=None, y=None):
         """Rows of x (plus residual, to sum_out) normalised, times w, to Q8_K
         rows and, where y is given, floats (c2h_rmsnorm_q8k_dev)."""
-        self._chk(lib().c2h_rmsnorm_q8k_dev(
-            self.h, ggml_type, x.data_ptr(), x.stride(0), _dp(residual), residual.stride(0) if residual is not None else 0,
-            w.data_ptr(), eps, x.shape[0], x.shape[1], _dp(sum_out), sum_out.stride(0) if sum_out is not None else 0,
-            q8k.data_ptr(), _dp(y), y.stride(0) if y is not None else 0))
+        n, cols = x.shape
+        rp, rs = (residual.data_ptr(), residual.stride(0)) if residual is not None else (None, 0)
+        sp, ss = (sum_out.data_ptr(), sum_out.stride(0)) if sum_out is not None else (None, 0)
+        yp, ys = (y.data_ptr(), y.stride(0)) if y is not None else (None, 0)
+        rc = _lib.c2h_rmsnorm_q8k_dev(self.h, ggml_type, x.data_ptr(), x.stride(0), rp, rs, w.data_ptr(), eps, n, cols, sp,
+                                      ss, q8k.data_ptr(), yp, ys)
+        if rc:
+            self._chk(rc)
 
 
 def _dp(t):

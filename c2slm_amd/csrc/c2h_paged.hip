@@ -72,25 +72,31 @@ __device__ __forceinline__ float2 cos_sin(const RopeTab& r, int i, int pos) {
 
 // Where a call's token goes: its position, and the byte offset of its slot
 // in the pool; false if it goes nowhere.  One whole wave: its lanes look for
-// the last session that starts at or before t, 64 starts a round.
+// the last session that starts at or before t, 64 starts a round, and the last
+// round brings the session's end and length with its start.
 __device__ __forceinline__ bool place(const RopeParams& P, int t, int* pos, int64_t* off) {
   const int lane = threadIdx.x & 63;
-  int s = t;
+  int s = t, len;
   int64_t end = (int64_t)t + 1;
   if (P.token_start) {
     int lo = 0, n = P.b.n_seqs;
-    while (n > 1) {
+    while (n > 64) {
       const int step = (n + 63) >> 6;
       const bool before = lane * step < n && P.token_start[lo + lane * step] <= t;
       const int skip = max((int)__popcll(__ballot(before)) - 1, 0) * step;
       lo += skip;
       n = min(step, n - skip);
     }
-    s = lo;
-    end = P.token_start[s + 1];
+    const int mine = lo + min(lane, n - 1);
+    const int first = P.token_start[mine], after = P.token_start[mine + 1], held = P.b.lens[mine];
+    const int at = max((int)__popcll(__ballot(lane < n && first <= t)) - 1, 0);
+    s = lo + at;
+    end = __builtin_amdgcn_readlane(after, at);
+    len = __builtin_amdgcn_readlane(held, at);
     if (t >= end) return false;
+  } else {
+    len = P.b.lens[s];
   }
-  const int len = P.b.lens[s];
   if (len == 0) return false;
   const int64_t p = token_pos(len, t, end);
   if (!length_ok(len, P.b.max_len) || p < 0) {
@@ -153,13 +159,17 @@ struct Run {
   }
 };
 
-// A workgroup takes P.tok consecutive tokens, up to four.  Wave w finds token
-// w's place and fills its cosines and sines (one 64-bit angle per pair and
+// A workgroup takes P.tok consecutive tokens, up to four.  A wave finds a
+// token's place and fills its cosines and sines (one 64-bit angle per pair and
 // token, in LDS for all heads); then every thread moves pairs of VEC-element
 // runs: the two halves of VEC rotated pairs in the half layout, neighbours
 // elsewhere, 16 bytes a load at 16 bits.  The first pair's loads are issued
-// before the angles, which they do not wait for.  Bound by memory: a step of
-// few tokens by its chain of loads (length, page) and the launch.
+// before the angles, which they do not wait for.
+// Bound by memory: 16,384 tokens of 32 heads of 128 (268 MB) 50.4 us, 5.3
+// TB/s, where a thread per pair with angles of its own took 151; 92 MB of
+// prompts into e4m3 23.5 us, 3.9 TB/s, of which the chain of loads before a
+// workgroup's first store (session, page) is the rest.  A step of few tokens
+// is that chain: 2.7 us for a rotation, 4.6 for 256 sessions' append.
 template <int T, int CT, bool CACHED, int VEC>
 __global__ void __launch_bounds__(256) k_rope(RopeParams P) {
   __shared__ float2 cs[ROPE_TOKENS][128];
@@ -209,16 +219,16 @@ __global__ void __launch_bounds__(256) k_rope(RopeParams P) {
   };
   load(x);
 
-  if (wave < tok) {
+  for (int tt = wave; tt < tok; tt += 4) {
     int pos = 0;
     int64_t off = 0;
     if constexpr (CACHED) {
-      if (!place(P, t0 + wave, &pos, &off)) off = -1;
-      if (lane == 0) slot[wave] = off;
+      if (!place(P, t0 + tt, &pos, &off)) off = -1;
+      if (lane == 0) slot[tt] = off;
     } else {
-      pos = P.positions[t0 + wave];
+      pos = P.positions[t0 + tt];
     }
-    for (int i = lane; i < half; i += 64) cs[wave][i] = cos_sin(R, i, pos);
+    for (int i = lane; i < half; i += 64) cs[tt][i] = cos_sin(R, i, pos);
   }
   __syncthreads();
 
@@ -949,8 +959,10 @@ void launch_rope_as(RopeParams P, hipStream_t st) {
   // x / d = (x * ceil(2^32 / d)) >> 32 for x up to 4 * rows * runs, far below 2^32 / d
   P.runs_magic = (uint32_t)(((1ull << 32) + P.runs - 1) / P.runs);
   P.rows_magic = (uint32_t)(((1ull << 32) + rows - 1) / rows);
-  // more tokens to a workgroup once there are enough workgroups without
-  P.tok = std::min(std::max(P.n_tokens / 1024, 1), ROPE_TOKENS);
+  // two items a thread once there are enough workgroups: 16,384 tokens of 32
+  // heads (256 items each) 50.4 us by two tokens, 53.2 by four, 53.8 by one;
+  // prompts into a pool of 2 KV heads (160 items) 24.7, 23.5 and 29.1
+  P.tok = std::min({std::max(P.n_tokens / 1024, 1), (511 + rows * P.runs) / (rows * P.runs), ROPE_TOKENS});
   const dim3 grid((P.n_tokens + P.tok - 1) / P.tok);
   if (narrow)
     hipLaunchKernelGGL((k_rope<T, CT, CACHED, 4>), grid, dim3(256), 0, st, P);
