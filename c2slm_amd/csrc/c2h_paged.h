@@ -54,20 +54,23 @@ C2H_HD constexpr int attn_tiles(int type, int hd) {
 }
 C2H_HD constexpr int attn_hd(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 C2H_HD constexpr int attn_unit(int type, int head_dim) { return 64 * attn_tiles(type, attn_hd(head_dim)); }
-// Units of a chunk whose pages a wave's lanes hold, one each.
-C2H_HD constexpr int most_units(int unit, int page_size) { return (64 - 1) * page_size / unit; }
 // Units per chunk: a batch of `units` in all, in each of n_rows (KV head, head
 // tile) rows, as about ATTN_CHUNKS equal chunks.
-C2H_HD inline int chunk_units(int64_t units, int n_rows, int most) {
+C2H_HD inline int chunk_units(int64_t units, int n_rows) {
   const int64_t c = (units * n_rows + ATTN_CHUNKS - 1) / ATTN_CHUNKS;
-  return (int)(c < 1 ? 1 : c > most ? most : c);
+  return (int)(c < 1 ? 1 : c);
 }
-// Chunks (of one row) that any batch can come to: about ATTN_CHUNKS / n_rows, and a
-// partial one per session, unless `most` cuts them shorter.
-inline int64_t chunks_bound(int n_seqs, int n_rows, int max_units, int most) {
-  const int64_t even = ATTN_CHUNKS / n_rows + 1 + n_seqs, cut = (int64_t)n_seqs * chunks_of(max_units, most);
-  const int64_t all = (int64_t)n_seqs * (max_units > 1 ? max_units : 1), b = even > cut ? even : cut;
-  return b < all ? b : all;
+// Chunks (of one row) that any batch of sessions of up to max_units can come
+// to: about ATTN_CHUNKS / n_rows, and a partial one per session.
+inline int64_t chunks_bound(int n_seqs, int n_rows, int max_units) {
+  const int64_t even = ATTN_CHUNKS / n_rows + 1 + n_seqs, all = (int64_t)n_seqs * (max_units > 1 ? max_units : 1);
+  return even < all ? even : all;
+}
+// A wave's lanes hold the pages from page p0 on, one each, enough for its
+// steps at base, base + unit, ... before the one returned.
+C2H_HD inline int first_step_beyond(int p0, int page_shift, int base, int step, int unit) {
+  const int limit = (p0 + 64) << page_shift;
+  return base + ((limit - step - base) / unit + 1) * unit;
 }
 
 C2H_HD inline bool length_ok(int len, int max_len) { return len >= 0 && len <= max_len; }
@@ -105,7 +108,6 @@ struct PagedAttnParams {
   int n_heads, group, n_tiles;  // query heads, per KV head, workgroups of ATTN_HEADS of them
   int window;
   int n_rows;                   // n_kv_heads * n_tiles
-  int most;                     // units of a chunk at most
   int grid;                     // workgroups
   float scale_log2;             // scale * log2(e)
   float* part_o;   // [chunks_bound][n_heads][head_dim]: sums of a chunk

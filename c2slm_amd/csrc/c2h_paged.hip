@@ -455,7 +455,7 @@ __device__ __forceinline__ int session_units(int len, int max_len, int window) {
   return units_of(attended(length_ok(len, max_len) ? len : 0, window), UNIT);
 }
 template <int UNIT>
-__device__ __forceinline__ Cut cut_batch(const int32_t* lens, int n_seqs, int max_len, int window, int n_rows, int most,
+__device__ __forceinline__ Cut cut_batch(const int32_t* lens, int n_seqs, int max_len, int window, int n_rows,
                                          bool split) {
   const int lane = threadIdx.x & 63;
   Cut c{(n_seqs + 63) >> 6, 1, 0, 0, n_seqs};
@@ -472,7 +472,7 @@ __device__ __forceinline__ Cut cut_batch(const int32_t* lens, int n_seqs, int ma
     }
     for (int m = 0; m < 64; ++m) units += __builtin_amdgcn_readlane(mine, m);
   }
-  c.units = chunk_units(units, n_rows, most);
+  c.units = chunk_units(units, n_rows);
   int n = 0;
   if (c.per == 1) {
     n = lane < n_seqs ? chunks_of(session_units<UNIT>(c.len, max_len, window), c.units) : 0;
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, j = lane >> 4;
   const int shift = shape & 255, n_tiles = shape >> 16;
   const bool split = shape & 256;
-  const Cut cut = cut_batch<A::UNIT>(lens, n_seqs, max_len, window, P.n_rows, P.most, split);
+  const Cut cut = cut_batch<A::UNIT>(lens, n_seqs, max_len, window, P.n_rows, split);
   const int csize = cut.units * A::UNIT, items = cut.total * P.n_rows;
 
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
@@ -539,14 +539,19 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   const Span span = attended(ok ? len : 0, window);
   const int n = chunks_of(units_of(span, A::UNIT), cut.units);
   const int base0 = chunk_base(span, csize, chunk), c0 = max(base0, span.lo), c1 = min(base0 + csize, span.hi);
-  const int p0 = c0 >> shift, last = c1 - 1;
+  const int last = c1 - 1;
   if (split && row == 0 && chunk == 0 && tid == 0) {
     P.info[2 * s] = unit;
     P.info[2 * s + 1] = n;
   }
-  // lane i holds page p0 + i: a chunk has at most 64
-  const bool paged = lane <= (last >> shift) - p0 && c1 > c0;
-  const int page = paged ? table[s * table_stride + p0 + lane] : 0;
+  // lane i holds page p0 + i, and the next 64 that the wave's steps come to
+  // are on their way
+  const int first = base0 + wave * A::STEP;  // the wave's steps: first, first + UNIT, ...
+  int p0 = c0 >> shift, beyond = first_step_beyond(p0, shift, first, A::STEP, A::UNIT);
+  auto held_pages = [&](int from) { return from + lane <= last >> shift && c1 > c0; };
+  auto load_pages = [&](int from) { return held_pages(from) ? table[s * table_stride + from + lane] : 0; };
+  const int page = load_pages(p0);
+  int next_page = beyond < c1 ? load_pages(beyond >> shift) : 0;
 
   const int kvh = n_tiles == 1 ? row : row / n_tiles;
   const int h0 = kvh * P.group + (row - kvh * n_tiles) * ATTN_HEADS;
@@ -563,8 +568,8 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
                 : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  const bool fail = !ok || __any(paged && !page_ok(page, P.kv.n_pages));
-  const int64_t page_off = page * P.kv.page_stride + kvh * P.kv.head_stride;
+  bool fail = !ok || __any(held_pages(p0) && !page_ok(page, P.kv.n_pages));
+  int64_t page_off = page * P.kv.page_stride + kvh * P.kv.head_stride;
 
   u32x4 K[NT][KC];
   uint32_t V[NT][4][NV][VW];
@@ -622,10 +627,10 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
       }
     }
   };
-  const bool work = !fail && base0 + wave * A::STEP < c1;
+  const bool work = !fail && first < c1;
   if (work) {
-    load_k(base0 + wave * A::STEP);
-    load_v(base0 + wave * A::STEP);
+    load_k(first);
+    load_v(first);
   }
 
   // the queries, split into the parts of the product
@@ -675,8 +680,9 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   float m = MINUS_INF, l = 0.0f;
 
   if (work) {
-    for (int base = base0 + wave * A::STEP; base < c1; base += 4 * A::STEP) {
-      const int next = base + 4 * A::STEP;
+    for (int base = first; base < c1; base += A::UNIT) {
+      // past the wave's last step its loads repeat that one, unused
+      const int next = base + A::UNIT < c1 ? base + A::UNIT : base;
       // scores
       f32x4 S[NT];
 #pragma unroll
@@ -700,6 +706,16 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
             }
           }
         }
+      if (next == beyond) {
+        p0 = beyond >> shift;
+        if (__any(held_pages(p0) && !page_ok(next_page, P.kv.n_pages))) {
+          fail = true;
+          break;
+        }
+        page_off = next_page * P.kv.page_stride + kvh * P.kv.head_stride;
+        beyond = first_step_beyond(p0, shift, next, A::STEP, A::UNIT);
+        next_page = beyond < c1 ? load_pages(beyond >> shift) : 0;
+      }
       load_k(next);
       // softmax
       const uint32_t at = (uint32_t)(base + 4 * j - c0), held = (uint32_t)(c1 - c0);
@@ -787,6 +803,13 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
     l = sum_of_rows(l);
   }
 
+  // A bad page or length: the wave's total is NaN, and so is the row.
+  if (fail) {
+    m = MINUS_INF;
+    l = __builtin_nanf("");
+    if (lane == 0) report(P.err, ok ? PERR_PAGE : PERR_LENGTH);
+  }
+
   // the waves' sums, brought to their common maximum, DB elements at a time
   if (lane < 16) {
     wm[wave][r] = m;
@@ -824,9 +847,8 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
         total += wl[w][head] * a;
         sum += *reinterpret_cast<const f32x4*>(os + (w * 16 + head) * A::OROW + d) * a;
       }
-      if (fail) sum = f32x4{0.0f, 0.0f, 0.0f, 0.0f} + __builtin_nanf("");
       if (n == 1) {
-        const float inv = fail ? 1.0f : total == 0.0f ? 0.0f : vs / total;
+        const float inv = total == 0.0f ? 0.0f : vs / total;
         store4(P.type, P.out.data + s * P.out.token_stride + (h0 + head) * P.out.head_stride +
                            (int64_t)(d0 + d) * (P.type == PT_F32 ? 4 : 2), sum * inv);
       } else {
@@ -839,7 +861,6 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
       }
     }
   }
-  if (fail && tid == 0) report(P.err, ok ? PERR_PAGE : PERR_LENGTH);
   }
 }
 

@@ -187,6 +187,37 @@ def test_attention_split_sessions(ctx, cache, ty, n):
     check_attention(ctx, [n, 1, 0, 700, n // 2], 14, 2, 64, 16, "hnd", cache, ty, seed=n)
 
 
+@pytest.mark.parametrize("cache,ty", [(H.F32, H.F32), (H.BF16, H.BF16), (H.F8_E4M3, H.F16)], ids=lambda t: NAMES[t])
+@pytest.mark.parametrize("window", [0, 1111])
+def test_attention_chunks_of_more_pages_than_lanes(ctx, cache, ty, window):
+    # 1,024 rows of up to 163 pages each, whole sessions by one workgroup: a
+    # wave's lanes hold 64 pages at a time
+    lens = [1300 - 7 * (i % 19) for i in range(62)] + [513, 1]
+    check_attention(ctx, lens, 16, 16, 16, 8, "nhd", cache, ty, window=window)
+
+
+def test_attention_bad_page_past_the_first_64(ctx):
+    lens = [1300] * 64
+    sess = Sessions(lens, 16, 16, 8, "nhd", H.F16, 9)
+    held = sess.table.clone()
+    sess.table[3, 100] = sess.n_pages
+    sess.table[9, 162] = -5
+    q = torch.randn(64, 16, 16, generator=torch.Generator().manual_seed(7)).half()
+    kv, batch = sess.cuda()
+    out, qd = torch.zeros_like(q, device="cuda"), q.cuda()
+    torch.cuda.synchronize()
+    ctx.paged_attn_dev(kv, batch, H.F16, 16, 0.25, H.heads(qd), H.heads(out))
+    with pytest.raises(H.C2hError) as e:
+        ctx.sync()
+    assert e.value.code == RANGE and "page" in str(e.value) and "length" not in str(e.value)
+    got = out.cpu().double()
+    assert torch.isnan(got[[3, 9]]).all()
+    sess.table = held
+    want, tol = attention64(sess, q, 0.25, 0, H.F16)
+    rest = [i for i in range(64) if i not in (3, 9)]
+    assert ((got - want).abs()[rest] <= tol[rest]).all()
+
+
 def test_attention_max_len_beyond_the_lengths(ctx):
     # the launch is sized by a bound far above the lengths: most chunks are empty
     sess = Sessions([5, 0, 300], 2, 64, 16, "nhd", H.F16, 3)

@@ -224,45 +224,55 @@ int main() {
          !page_ok(INT_MAX, 100));
   assert(length_ok(0, 0) && length_ok(5, 5) && !length_ok(6, 5) && !length_ok(-1, 5) && !length_ok(INT_MIN, 1 << 30));
   // windows and chunks cover the span once, in order, without overflow, and
-  // a chunk's pages are at most a wave's lanes
+  // a wave holds the pages of its steps
   const int lens[] = {0, 1, 2, 127, 128, 129, 4095, 4096, 100001, PAGED_MAX_LEN};
   const int wins[] = {0, 1, 127, 128, 1000, 1 << 30};
   for (int len : lens)
     for (int w : wins)
       for (int unit : {64, 128, 256})
-        for (int page = 8; page <= 1024; page *= 2)
-          for (int cu : {1, 2, 3, 7, most_units(unit, page)}) {
-            if (cu > most_units(unit, page)) continue;
-            const int chunk = cu * unit;
-            const Span s = attended(len, w);
-            assert(s.hi == len && s.lo >= 0 && s.hi - s.lo == (w > 0 && w < len ? w : len));
-            const int units = units_of(s, unit), n = chunks_of(units, cu);
-            const int longest = w > 0 && w < PAGED_MAX_LEN ? w + SPAN_ALIGN - 1 : PAGED_MAX_LEN;
-            assert(n >= 1 && (units == 0) == (len == 0) && units <= units_of(Span{0, longest}, unit));
-            int64_t at = s.lo;
-            for (int i = 0; len > 0 && i < n; i = i == 2 && n > 6 ? n - 3 : i + 1) {  // the first and last three
-              const int64_t b = chunk_base(s, chunk, i), c0 = b > s.lo ? b : s.lo, c1 = b + chunk < s.hi ? b + chunk : s.hi;
-              assert(b % SPAN_ALIGN == 0 && c1 > c0 && c1 - c0 <= chunk && (i < 3 ? c0 == at : c0 > s.lo));
-              at = c1;
-              assert((c1 - 1) / page - c0 / page < 64);
-            }
-            assert(at == s.hi);
+        for (int cu : {1, 2, 3, 7, 30, 1000}) {
+          const int chunk = cu * unit, step = unit / 4;
+          const Span s = attended(len, w);
+          assert(s.hi == len && s.lo >= 0 && s.hi - s.lo == (w > 0 && w < len ? w : len));
+          const int units = units_of(s, unit), n = chunks_of(units, cu);
+          const int longest = w > 0 && w < PAGED_MAX_LEN ? w + SPAN_ALIGN - 1 : PAGED_MAX_LEN;
+          assert(n >= 1 && (units == 0) == (len == 0) && units <= units_of(Span{0, longest}, unit));
+          int64_t at = s.lo;
+          for (int i = 0; len > 0 && i < n; i = i == 2 && n > 6 ? n - 3 : i + 1) {  // the first and last three
+            const int64_t b = chunk_base(s, chunk, i), c0 = b > s.lo ? b : s.lo, c1 = b + chunk < s.hi ? b + chunk : s.hi;
+            assert(b % SPAN_ALIGN == 0 && c1 > c0 && c1 - c0 <= chunk && (i < 3 ? c0 == at : c0 > s.lo));
+            at = c1;
+            for (int sh = 3; sh <= 10; ++sh)
+              for (int wave = 0; wave < 4; ++wave) {
+                int p0 = (int)c0 >> sh, first = (int)b + wave * step, beyond = first_step_beyond(p0, sh, first, step, unit);
+                int turns = 0;
+                for (int base = first; base < c1 && turns < 5; base += unit) {
+                  if (base == beyond) {
+                    p0 = base >> sh;
+                    beyond = first_step_beyond(p0, sh, base, step, unit);
+                    ++turns;
+                  }
+                  assert(base < beyond && (beyond - first) % unit == 0);
+                  for (int pos : {base, base + step - 1}) {
+                    const int p = pos < c0 ? (int)c0 : pos < c1 ? pos : (int)c1 - 1;
+                    assert((p >> sh) - p0 >= 0 && (p >> sh) - p0 < 64);
+                  }
+                }
+              }
           }
+          assert(at == s.hi);
+        }
   // the bound of a batch's chunks holds for even and uneven batches
   for (int n_seqs : {1, 2, 63, 64, 65, 700})
     for (int rows : {1, 2, 8, 600})
-      for (int most : {1, 4, 30})
-        for (int shape = 0; shape < 4; ++shape) {
-          int64_t units = 0, chunks = 0;
-          auto u = [&](int i) { return shape == 0 ? 0 : shape == 1 ? 50 : shape == 2 ? (i * 7919) % 51 : i ? 1 : 50; };
-          for (int i = 0; i < n_seqs; ++i) units += u(i);
-          const int cu = chunk_units(units, rows, most);
-          assert(cu >= 1 && cu <= most);
-          for (int i = 0; i < n_seqs; ++i) chunks += chunks_of(u(i), cu);
-          assert(chunks <= chunks_bound(n_seqs, rows, 50, most));
-        }
-  for (int type : {PT_F32, PT_F16, PT_BF16, PT_E4M3})
-    for (int hd = 16; hd <= 256; hd += 16) assert(most_units(attn_unit(type, hd), PAGED_MIN_PAGE) >= 1);
+      for (int shape = 0; shape < 4; ++shape) {
+        int64_t units = 0, chunks = 0;
+        auto u = [&](int i) { return shape == 0 ? 0 : shape == 1 ? 50 : shape == 2 ? (i * 7919) % 51 : i ? 1 : 50; };
+        for (int i = 0; i < n_seqs; ++i) units += u(i);
+        const int cu = chunk_units(units, rows);
+        for (int i = 0; i < n_seqs; ++i) chunks += chunks_of(u(i), cu);
+        assert(cu >= 1 && chunks <= chunks_bound(n_seqs, rows, 50));
+      }
   // the tokens of a session are its last ones
   assert(token_pos(10, 5, 6) == 9 && token_pos(10, 0, 6) == 4 && token_pos(3, 0, 6) == -3 && token_pos(0, 0, 1) == -1);
   assert(token_pos(1 << 30, INT_MAX - 1, INT_MAX) == (1 << 30) - 1);
