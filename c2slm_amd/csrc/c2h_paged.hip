@@ -488,8 +488,9 @@ __device__ __forceinline__ Cut cut_batch(const int32_t* lens, int n_seqs, int ma
 }
 
 // The leading arguments arrive in registers at wave start (kernel-argument
-// preload).  shape: log2 of the page size; bit 8: sessions can have several
-// chunks; n_tiles from bit 16.
+// preload).  shape: log2 of the page size; from bit 4: whether sessions can
+// have several chunks; from bit 5: n_tiles; from bit 14: n_kv_heads.
+using Args = const __attribute__((address_space(4))) PagedAttnParams*;
 template <int CT, int HD, bool FULL, bool PRECISE, bool STREAM>
 __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 : 2)
     k_paged_attn(const int32_t* lens, const int32_t* table, int64_t table_stride, int max_len, int window, uint32_t shape,
@@ -500,14 +501,22 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   __shared__ __align__(16) char lds[A::LDS];
   __shared__ float mul[16], wm[4][16], wl[4][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, j = lane >> 4;
-  const int shift = shape & 255, n_tiles = shape >> 16;
-  const bool split = shape & 256;
-  const Cut cut = cut_batch<A::UNIT>(lens, n_seqs, max_len, window, P.n_rows, split);
-  const int csize = cut.units * A::UNIT, items = cut.total * P.n_rows;
+  // the block behind the leading arguments, read where it is used: kept in
+  // registers over the loop below, its fields spill
+  auto fresh = [&]() {
+    Args a = (Args)((const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr() + 40), b;
+    asm volatile("" : "=s"(b) : "0"(a));
+    return b;
+  };
+  const int shift = shape & 15, n_tiles = (shape >> 5) & 511, n_rows = (shape >> 14) * n_tiles;
+  const bool split = shape & 16;
+  const Cut cut = cut_batch<A::UNIT>(lens, n_seqs, max_len, window, n_rows, split);
+  const int csize = cut.units * A::UNIT, items = cut.total * n_rows;
 
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
   // the item's session and chunk
-  const int unit = item / P.n_rows, row = item - unit * P.n_rows;
+  Args args = fresh();
+  const int unit = item / n_rows, row = item - unit * n_rows;
   int s = unit, chunk = 0, len = 0;
   if (!split) {
     len = lens[s];
@@ -541,8 +550,8 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   const int base0 = chunk_base(span, csize, chunk), c0 = max(base0, span.lo), c1 = min(base0 + csize, span.hi);
   const int last = c1 - 1;
   if (split && row == 0 && chunk == 0 && tid == 0) {
-    P.info[2 * s] = unit;
-    P.info[2 * s + 1] = n;
+    args->info[2 * s] = unit;
+    args->info[2 * s + 1] = n;
   }
   // lane i holds page p0 + i, and the next 64 that the wave's steps come to
   // are on their way
@@ -554,31 +563,32 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   int next_page = beyond < c1 ? load_pages(beyond >> shift) : 0;
 
   const int kvh = n_tiles == 1 ? row : row / n_tiles;
-  const int h0 = kvh * P.group + (row - kvh * n_tiles) * ATTN_HEADS;
-  const int nh = min(ATTN_HEADS, (kvh + 1) * P.group - h0);
-  const int hd = FULL ? HD : P.kv.head_dim;
+  const int h0 = kvh * args->group + (row - kvh * n_tiles) * ATTN_HEADS;
+  const int nh = min(ATTN_HEADS, (kvh + 1) * args->group - h0);
+  const int hd = FULL ? HD : args->kv.head_dim;
   constexpr int EPT = HD / 16;  // elements of the queries that a thread brings
   const int qhead = tid >> 4, qd0 = (tid & 15) * EPT;
   f32x4 q[EPT / 4];
 #pragma unroll
   for (int g = 0; g < EPT / 4; ++g) {
     const bool have = qhead < nh && (FULL || qd0 + 4 * g < hd);
-    q[g] = have ? load4(P.type, P.q.data + s * P.q.token_stride + (h0 + qhead) * P.q.head_stride +
-                                    (int64_t)(qd0 + 4 * g) * (P.type == PT_F32 ? 4 : 2))
+    q[g] = have ? load4(args->type, args->q.data + s * args->q.token_stride + (h0 + qhead) * args->q.head_stride +
+                                    (int64_t)(qd0 + 4 * g) * (args->type == PT_F32 ? 4 : 2))
                 : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  bool fail = !ok || __any(held_pages(p0) && !page_ok(page, P.kv.n_pages));
-  int64_t page_off = page * P.kv.page_stride + kvh * P.kv.head_stride;
+  bool fail = !ok || __any(held_pages(p0) && !page_ok(page, args->kv.n_pages));
+  int64_t page_off = page * args->kv.page_stride + kvh * args->kv.head_stride;
 
   u32x4 K[NT][KC];
   uint32_t V[NT][4][NV][VW];
   const int rowb = hd * A::ES, mask = (1 << shift) - 1;
-  const uint32_t ts = (uint32_t)P.kv.token_stride;  // below 2^31
+  const uint32_t ts = (uint32_t)args->kv.token_stride;  // below 2^31
   // Positions outside [c0, c1) are read as the nearest inside, and masked
   // in the scores; elements past head_dim as the row's first, against zeros
   // of Q and into output tiles that are not stored.
-  auto inside = [&](int pos) { return min(max(pos, c0), last); };
+  int from = c0, to = last;
+  auto inside = [&](int pos) { return min(max(pos, from), to); };
   auto page_of = [&](int pos) {
     const int at = ((pos >> shift) - p0) * 4;
     const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_bpermute(at, (int)page_off);
@@ -590,7 +600,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int pos = inside(base + 16 * t + r);
-      const char* row = P.kv.k + page_of(pos) + in_page(pos);
+      const char* row = args->kv.k + page_of(pos) + in_page(pos);
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         int off = c * 64 + j * 16;
@@ -604,7 +614,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
     for (int t = 0; t < NT; ++t) {
       // one page holds those of the four positions that are inside
       const int first = base + 16 * t + 4 * j;
-      const char* at = P.kv.v + page_of(inside(first));
+      const char* at = args->kv.v + page_of(inside(first));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const char* row = at + in_page(inside(first + i));
@@ -650,8 +660,8 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
       }
     }
     if ((tid & 15) == 0) {
-      const float ks = A::F8 && P.kv.k_scale ? P.kv.k_scale[kvh] : 1.0f;
-      mul[qhead] = ldexpf(P.scale_log2 * ks, -e);
+      const float ks = A::F8 && args->kv.k_scale ? args->kv.k_scale[kvh] : 1.0f;
+      mul[qhead] = ldexpf(args->scale_log2 * ks, -e);
     }
 #pragma unroll
     for (int g = 0; g < EPT / 4; ++g) {
@@ -681,8 +691,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
 
   if (work) {
     for (int base = first; base < c1; base += A::UNIT) {
-      // past the wave's last step its loads repeat that one, unused
-      const int next = base + A::UNIT < c1 ? base + A::UNIT : base;
+      const int next = base + A::UNIT;
       // scores
       f32x4 S[NT];
 #pragma unroll
@@ -706,16 +715,18 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
             }
           }
         }
-      if (next == beyond) {
+      if (next == beyond && next < c1) {
+        Args pool = fresh();
         p0 = beyond >> shift;
-        if (__any(held_pages(p0) && !page_ok(next_page, P.kv.n_pages))) {
+        if (__any(held_pages(p0) && !page_ok(next_page, pool->kv.n_pages))) {
           fail = true;
           break;
         }
-        page_off = next_page * P.kv.page_stride + kvh * P.kv.head_stride;
+        page_off = next_page * pool->kv.page_stride + kvh * pool->kv.head_stride;
         beyond = first_step_beyond(p0, shift, next, A::STEP, A::UNIT);
         next_page = beyond < c1 ? load_pages(beyond >> shift) : 0;
       }
+      if (next >= c1) from = to = max(base, c0);  // no next step: one row, unused
       load_k(next);
       // softmax
       const uint32_t at = (uint32_t)(base + 4 * j - c0), held = (uint32_t)(c1 - c0);
@@ -803,11 +814,12 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
     l = sum_of_rows(l);
   }
 
+  Args at_end = fresh();
   // A bad page or length: the wave's total is NaN, and so is the row.
   if (fail) {
     m = MINUS_INF;
     l = __builtin_nanf("");
-    if (lane == 0) report(P.err, ok ? PERR_PAGE : PERR_LENGTH);
+    if (lane == 0) report(at_end->err, ok ? PERR_PAGE : PERR_LENGTH);
   }
 
   // the waves' sums, brought to their common maximum, DB elements at a time
@@ -816,7 +828,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
     wl[wave][r] = l;
   }
   float* os = reinterpret_cast<float*>(lds);
-  const float vs = A::F8 && P.kv.v_scale ? P.kv.v_scale[kvh] : 1.0f;
+  const float vs = A::F8 && at_end->kv.v_scale ? at_end->kv.v_scale[kvh] : 1.0f;
 #pragma unroll
   for (int d0 = 0; d0 < HD; d0 += A::DB) {
     __syncthreads();  // the queries, or the elements before, are read
@@ -849,14 +861,14 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
       }
       if (n == 1) {
         const float inv = total == 0.0f ? 0.0f : vs / total;
-        store4(P.type, P.out.data + s * P.out.token_stride + (h0 + head) * P.out.head_stride +
-                           (int64_t)(d0 + d) * (P.type == PT_F32 ? 4 : 2), sum * inv);
+        store4(at_end->type, at_end->out.data + s * at_end->out.token_stride + (h0 + head) * at_end->out.head_stride +
+                           (int64_t)(d0 + d) * (at_end->type == PT_F32 ? 4 : 2), sum * inv);
       } else {
-        const int64_t part = (int64_t)unit * P.n_heads + h0 + head;
-        *reinterpret_cast<f32x4*>(P.part_o + part * hd + d0 + d) = sum * vs;
+        const int64_t part = (int64_t)unit * at_end->n_heads + h0 + head;
+        *reinterpret_cast<f32x4*>(at_end->part_o + part * hd + d0 + d) = sum * vs;
         if (d0 + d == 0) {
-          P.part_ml[part * 2] = top;
-          P.part_ml[part * 2 + 1] = total;
+          at_end->part_ml[part * 2] = top;
+          at_end->part_ml[part * 2 + 1] = total;
         }
       }
     }
@@ -928,7 +940,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const int32_t* info, const f
 
 template <int CT, int HD, bool FULL, bool PRECISE, bool STREAM>
 void launch_attn_as(const PagedAttnParams& P, hipStream_t st) {
-  const uint32_t shape = (uint32_t)P.kv.page_shift | (P.info ? 256u : 0u) | (uint32_t)P.n_tiles << 16;
+  const uint32_t shape = (uint32_t)P.kv.page_shift | (P.info ? 16u : 0u) | (uint32_t)P.n_tiles << 5 | (uint32_t)P.kv.n_kv_heads << 14;
   hipLaunchKernelGGL((k_paged_attn<CT, HD, FULL, PRECISE, STREAM>), dim3(P.grid), dim3(256), 0, st, P.b.lens, P.b.table,
                      P.b.table_stride, P.b.max_len, P.window, shape, P.b.n_seqs, P);
   if (P.info)
