@@ -2867,13 +2867,11 @@ int c2h_rmsnorm_q8k_dev(c2h_ctx* c, int32_t type, const void* x, int64_t x_strid
                         int64_t sum_stride, void* q8k_out, float* y_out, int64_t y_stride) {
   if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
   if (n_rows < 0) return fail(c, C2H_ERR_INVALID, "%d rows", n_rows);
-  if (cols < 256 || cols > 16384 || cols % 8)
-    return fail(c, C2H_ERR_UNSUPPORTED, "%d columns: a multiple of 8 from 256 to 16384", cols);
+  if (cols < 256 || cols > 16384) return fail(c, C2H_ERR_UNSUPPORTED, "%d columns: 256 to 16384", cols);
   if (n_rows > 0 && (!x || !w || !q8k_out || (residual != nullptr) != (sum_out != nullptr)))
     return fail(c, C2H_ERR_INVALID, "x, w and q8k_out are required, residual and sum_out come together");
   if (!(eps >= 0.0f)) return fail(c, C2H_ERR_INVALID, "eps from 0");
   const int es = type_bytes(type);
-  uintptr_t low = reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(y_out);
   const struct {
     const void* p;
     int64_t stride;
@@ -2885,10 +2883,10 @@ int c2h_rmsnorm_q8k_dev(c2h_ctx* c, int32_t type, const void* x, int64_t x_strid
     if (!r.p) continue;
     if (!stride_fits(r.stride, n_rows, r.es) || (r.written && n_rows > 1 && r.stride < cols))
       return fail(c, C2H_ERR_INVALID, "a row stride of %lld elements for %d columns", (long long)r.stride, cols);
-    low |= reinterpret_cast<uintptr_t>(r.p) | (uintptr_t)(r.stride * r.es);
+    if (reinterpret_cast<uintptr_t>(r.p) % r.es) return fail(c, C2H_ERR_INVALID, "rows start at whole elements");
   }
-  if ((low & 15) || (reinterpret_cast<uintptr_t>(q8k_out) & 3))
-    return fail(c, C2H_ERR_INVALID, "rows and w must be multiples of 16 bytes, q8k_out of 4");
+  if ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(q8k_out)) & 3)
+    return fail(c, C2H_ERR_INVALID, "w and q8k_out must be multiples of 4 bytes");
   if (!c) return fail(c, C2H_ERR_INVALID, "no context");
   if (n_rows == 0) return C2H_OK;
   HIPCHK(c, hipSetDevice(c->device));

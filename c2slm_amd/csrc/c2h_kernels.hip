@@ -516,10 +516,20 @@ struct Q8KOut {
         d{reinterpret_cast<float*>(y)} {}
 };
 
-// Elements 4i .. 4i+3 of a row.
-template <int T>
-__device__ __forceinline__ float4 load_row4(const char* row, int i) {
-  if constexpr (T == PT_F32) {
+// Elements 4i .. 4i+3 of a row of cols elements (0 from cols on).  VEC: rows
+// and cols are multiples of four elements, which move as one.
+template <int T, bool VEC>
+__device__ __forceinline__ float4 load_row4(const char* row, int i, int cols) {
+  if (4 * i >= cols) return make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if constexpr (!VEC) {
+    auto at = [&](int e) {
+      if (e >= cols) return 0.0f;
+      if constexpr (T == PT_F32) return reinterpret_cast<const float*>(row)[e];
+      if constexpr (T == PT_F16) return (float)reinterpret_cast<const _Float16*>(row)[e];
+      return (float)reinterpret_cast<const __bf16*>(row)[e];
+    };
+    return make_float4(at(4 * i), at(4 * i + 1), at(4 * i + 2), at(4 * i + 3));
+  } else if constexpr (T == PT_F32) {
     return reinterpret_cast<const float4*>(row)[i];
   } else {
     const uint2 u = reinterpret_cast<const uint2*>(row)[i];
@@ -531,9 +541,18 @@ __device__ __forceinline__ float4 load_row4(const char* row, int i) {
   }
 }
 // Stores v rounded to the type and returns what was stored.
-template <int T>
-__device__ __forceinline__ float4 store_row4(char* row, int i, float4 v) {
-  if constexpr (T == PT_F32) {
+template <int T, bool VEC>
+__device__ __forceinline__ float4 store_row4(char* row, int i, int cols, float4 v) {
+  if (4 * i >= cols) return v;
+  if constexpr (!VEC) {
+    auto at = [&](int e, float x) {
+      if (e >= cols) return 0.0f;
+      if constexpr (T == PT_F32) return reinterpret_cast<float*>(row)[e] = x;
+      if constexpr (T == PT_F16) return (float)(reinterpret_cast<_Float16*>(row)[e] = (_Float16)x);
+      return (float)(reinterpret_cast<__bf16*>(row)[e] = (__bf16)x);
+    };
+    return make_float4(at(4 * i, v.x), at(4 * i + 1, v.y), at(4 * i + 2, v.z), at(4 * i + 3, v.w));
+  } else if constexpr (T == PT_F32) {
     reinterpret_cast<float4*>(row)[i] = v;
     return v;
   } else if constexpr (T == PT_F16) {
@@ -553,7 +572,12 @@ __device__ __forceinline__ float4 store_row4(char* row, int i, float4 v) {
 // ... (BPW of them), lane l elements 4l .. 4l+3 of each, as quantize_blocks
 // takes them; the row is read once and stays in registers.  The squares are
 // summed in 64 bits, so that the order of the sum does not reach the quants.
-template <int T, int BPW, int NW>
+// Bound by memory: 8,192 rows of 2,048 bf16 with residual, quants and f32 rows
+// (187 MB) 39.8 us, 4.7 TB/s, what a large copy reaches; one row of 896 is 2.3
+// us, launch and one chain of loads.  Tried: streamed loads 38.3 (but x is
+// fresh in the caches where a layer runs), the weights loaded before the sum
+// 40.3.
+template <int T, int BPW, int NW, bool VEC>
 __global__ void __launch_bounds__(64 * NW) k_norm_q8(NormQ8Params P) {
   __shared__ double part[NW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -561,20 +585,15 @@ __global__ void __launch_bounds__(64 * NW) k_norm_q8(NormQ8Params P) {
   const char* x = P.x + row * P.x_stride;
   float4 v[BPW];
 #pragma unroll
-  for (int i = 0; i < BPW; ++i) {
-    const int c4 = (wave + NW * i) * 64 + lane;
-    v[i] = 4 * c4 < P.cols ? load_row4<T>(x, c4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  }
+  for (int i = 0; i < BPW; ++i) v[i] = load_row4<T, VEC>(x, (wave + NW * i) * 64 + lane, P.cols);
   if (P.r) {
     const char* r = P.r + row * P.r_stride;
     char* sum = P.sum + row * P.sum_stride;
 #pragma unroll
     for (int i = 0; i < BPW; ++i) {
       const int c4 = (wave + NW * i) * 64 + lane;
-      if (4 * c4 < P.cols) {
-        const float4 a = load_row4<T>(r, c4);
-        v[i] = store_row4<T>(sum, c4, make_float4(v[i].x + a.x, v[i].y + a.y, v[i].z + a.z, v[i].w + a.w));
-      }
+      const float4 a = load_row4<T, VEC>(r, c4, P.cols);
+      v[i] = store_row4<T, VEC>(sum, c4, P.cols, make_float4(v[i].x + a.x, v[i].y + a.y, v[i].z + a.z, v[i].w + a.w));
     }
   }
   double ss = 0.0;
@@ -592,11 +611,9 @@ __global__ void __launch_bounds__(64 * NW) k_norm_q8(NormQ8Params P) {
 #pragma unroll
   for (int i = 0; i < BPW; ++i) {
     const int c4 = (wave + NW * i) * 64 + lane;
-    if (4 * c4 < P.cols) {
-      const float4 w = reinterpret_cast<const float4*>(P.w)[c4];
-      v[i] = make_float4((v[i].x * scale) * w.x, (v[i].y * scale) * w.y, (v[i].z * scale) * w.z, (v[i].w * scale) * w.w);
-      if (P.y) reinterpret_cast<float4*>(P.y + row * P.y_stride)[c4] = v[i];
-    }
+    const float4 w = load_row4<PT_F32, VEC>(reinterpret_cast<const char*>(P.w), c4, P.cols);
+    v[i] = make_float4((v[i].x * scale) * w.x, (v[i].y * scale) * w.y, (v[i].z * scale) * w.z, (v[i].w * scale) * w.w);
+    if (P.y) store_row4<PT_F32, VEC>(reinterpret_cast<char*>(P.y + row * P.y_stride), c4, P.cols, v[i]);
   }
   const int nb = P.cols / QK_K;
   Q8KOut out(P.q8k + row * nb * BS_Q8K);
@@ -604,30 +621,41 @@ __global__ void __launch_bounds__(64 * NW) k_norm_q8(NormQ8Params P) {
 }
 
 namespace {
-template <int T>
+template <int T, bool VEC>
 void launch_norm_q8_t(const NormQ8Params& P, hipStream_t st) {
   const int nbt = (P.cols + QK_K - 1) / QK_K;
   const dim3 grid(P.n_rows);
   if (nbt <= 4)
-    hipLaunchKernelGGL((k_norm_q8<T, 1, 4>), grid, dim3(256), 0, st, P);
+    hipLaunchKernelGGL((k_norm_q8<T, 1, 4, VEC>), grid, dim3(256), 0, st, P);
   else if (nbt <= 8)
-    hipLaunchKernelGGL((k_norm_q8<T, 2, 4>), grid, dim3(256), 0, st, P);
+    hipLaunchKernelGGL((k_norm_q8<T, 2, 4, VEC>), grid, dim3(256), 0, st, P);
   else if (nbt <= 16)
-    hipLaunchKernelGGL((k_norm_q8<T, 4, 4>), grid, dim3(256), 0, st, P);
+    hipLaunchKernelGGL((k_norm_q8<T, 4, 4, VEC>), grid, dim3(256), 0, st, P);
   else if (nbt <= 32)
-    hipLaunchKernelGGL((k_norm_q8<T, 4, 8>), grid, dim3(512), 0, st, P);
+    hipLaunchKernelGGL((k_norm_q8<T, 4, 8, VEC>), grid, dim3(512), 0, st, P);
   else
-    hipLaunchKernelGGL((k_norm_q8<T, 4, 16>), grid, dim3(1024), 0, st, P);
+    hipLaunchKernelGGL((k_norm_q8<T, 4, 16, VEC>), grid, dim3(1024), 0, st, P);
+}
+template <int T>
+void launch_norm_q8_v(const NormQ8Params& P, int type, hipStream_t st) {
+  // four elements at a time where every row starts at a multiple of four
+  const uint64_t four = 4 * type_bytes(type), rows = (uint64_t)P.x | (uint64_t)P.r | (uint64_t)P.sum | (uint64_t)P.x_stride |
+                                                     (uint64_t)P.r_stride | (uint64_t)P.sum_stride;
+  const bool vec = P.cols % 4 == 0 && rows % four == 0 && ((uint64_t)P.w | (uint64_t)P.y) % 16 == 0 && P.y_stride % 4 == 0;
+  if (vec)
+    launch_norm_q8_t<T, true>(P, st);
+  else
+    launch_norm_q8_t<T, false>(P, st);
 }
 }  // namespace
 
 void launch_norm_q8(const NormQ8Params& P, int type, hipStream_t st) {
   if (type == PT_F32)
-    launch_norm_q8_t<PT_F32>(P, st);
+    launch_norm_q8_v<PT_F32>(P, type, st);
   else if (type == PT_F16)
-    launch_norm_q8_t<PT_F16>(P, st);
+    launch_norm_q8_v<PT_F16>(P, type, st);
   else
-    launch_norm_q8_t<PT_BF16>(P, st);
+    launch_norm_q8_v<PT_BF16>(P, type, st);
 }
 
 // rms_scale against the IEEE operations over the bit patterns [lo, lo + n);

@@ -415,8 +415,7 @@ int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* batc
                              size_t* bytes);
 
 /* RMSNorm with the residual's addition and Q8_K rows as its output: for each
- * of n_rows rows of cols elements (256 .. 16384, a multiple of 8) of `type`
- * (F32, F16, BF16)
+ * of n_rows rows of cols elements (256 .. 16384) of `type` (F32, F16, BF16)
  *   s = x + residual (rounded to the type and stored to sum_out; s = x where
  *       residual is NULL),
  *   y = (s * f32(1 / sqrt(mean(s^2) + eps))) * w,
@@ -426,8 +425,8 @@ int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* batc
  * bytes).  y_out (nullable) receives y as floats, all cols of it, for the
  * formats whose products read f32 rows.  Rows of x, residual and sum_out are
  * x_stride, residual_stride and sum_stride elements apart, those of y_out
- * y_stride floats; pointers and strides are multiples of 16 bytes (q8k_out:
- * 4).  sum_out is required with a residual (NULL without) and may be x or
+ * y_stride floats; any alignment of whole elements (q8k_out: 4 bytes), rows
+ * and cols of multiples of four elements being the faster ones.  sum_out is required with a residual (NULL without) and may be x or
  * the residual itself (same pointer and stride). */
 int c2h_rmsnorm_q8k_dev(c2h_ctx* ctx, int32_t type, const void* x, int64_t x_stride, const void* residual,
                         int64_t residual_stride, const float* w, float eps, int32_t n_rows, int32_t cols,

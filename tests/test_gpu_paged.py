@@ -565,6 +565,36 @@ def test_norm(ctx, ty, rows, cols):
             assert (yo[rows:] == 4.0).all() and (yo[:, cols:] == 4.0).all() and (want_y or (yo == 4.0).all())
 
 
+@pytest.mark.parametrize("ty", [H.F32, H.F16, H.BF16], ids=lambda t: NAMES[t])
+@pytest.mark.parametrize("rows,cols,shift", [(3, 257, 0), (2, 434, 0), (4, 1001, 0), (2, 2047, 0), (1, 5003, 0), (1, 16383, 0),
+                                             (3, 896, 1), (2, 1024, 2)])
+def test_norm_odd_widths_and_alignments(ctx, ty, rows, cols, shift):
+    # packed rows of odd widths; even ones that start between fours
+    g = torch.Generator().manual_seed(cols)
+    flat = [torch.randn(rows * cols + 8, generator=g).to(TORCH[ty]) for _ in range(2)]
+    x, r = (f[shift:shift + rows * cols].view(rows, cols) for f in flat)
+    w = torch.rand(cols + 4, generator=g)[shift:shift + cols]
+    s, y = norm_expect(x, r, w, 1e-5, ty)
+    fd = [f.cuda() for f in flat]
+    xd, rd = (f[shift:shift + rows * cols].view(rows, cols) for f in fd)
+    wd = torch.nn.functional.pad(w, (shift, 4)).cuda()[shift:shift + cols]
+    nb = cols // 256
+    q8k = torch.full((rows * nb * 292 + 8,), 0xAB, dtype=torch.uint8, device="cuda")
+    so = torch.full((rows * cols + 8,), 4.0, dtype=TORCH[ty], device="cuda")
+    yo = torch.full((rows * cols + 8,), 4.0, device="cuda")
+    sv, yv = (t[shift:shift + rows * cols].view(rows, cols) for t in (so, yo))
+    torch.cuda.synchronize()
+    ctx.rmsnorm_q8k_dev(ty, xd, wd, 1e-5, q8k, residual=rd, sum_out=sv, y=yv)
+    ctx.sync()
+    got = q8k.cpu().numpy()
+    for i in range(rows):
+        assert np.array_equal(got[i * nb * 292:(i + 1) * nb * 292], O.quantize_row_q8k(y[i].numpy())), i
+    assert (got[rows * nb * 292:] == 0xAB).all()
+    assert torch.equal(sv.cpu(), s) and torch.equal(yv.cpu(), y)
+    for t in (so, yo):
+        assert (t[:shift] == 4.0).all() and (t[shift + rows * cols:] == 4.0).all(), "elements beside the rows changed"
+
+
 def test_norm_in_place_zero_rows_and_special_values(ctx):
     g = torch.Generator().manual_seed(5)
     x, r, w = torch.randn(4, 896, generator=g), torch.randn(4, 896, generator=g), torch.ones(896)

@@ -142,7 +142,7 @@ def test_norm_arguments_refused():
         return L.c2h_rmsnorm_q8k_dev(None, type, x, xs, r, rs, w, eps, n, cols, s, ss, q, y, ys)
 
     refused(norm(type=H.F8_E4M3), UNSUPPORTED, "type")
-    for cols in (248, 0, -256, 900, 16392):
+    for cols in (255, 0, -256, 16385):
         refused(norm(cols=cols), UNSUPPORTED, "columns")
     refused(norm(n=-1), INVALID, "rows")
     refused(norm(x=None), INVALID, "required")
@@ -152,9 +152,12 @@ def test_norm_arguments_refused():
     refused(norm(s=A, ss=1024), INVALID, "come together")
     refused(norm(eps=-1.0), INVALID, "eps")
     refused(norm(eps=float("nan")), INVALID, "eps")
-    refused(norm(x=A + 4), INVALID, "16 bytes")
-    refused(norm(xs=898), INVALID, "16 bytes")
-    refused(norm(q=A + 2), INVALID, "q8k_out of 4")
+    refused(norm(x=A + 2), INVALID, "whole elements")
+    refused(norm(type=H.BF16, x=A + 1), INVALID, "whole elements")
+    refused(norm(y=A + 2, ys=1024), INVALID, "whole elements")
+    refused(norm(q=A + 2), INVALID, "q8k_out must be")
+    refused(norm(w=A + 1), INVALID, "4 bytes")
+    refused(norm(type=H.BF16, x=A + 2, xs=897, cols=897), INVALID, "no context")
     refused(norm(y=A, ys=512), INVALID, "row stride")
     refused(norm(r=A, rs=1024, s=A, ss=0), INVALID, "row stride")
     refused(norm(xs=-1024), INVALID, "row stride")
