@@ -2690,7 +2690,7 @@ int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int 
   // a window's first position may add up to three to its span
   const int span = window > 0 && window < b->max_len ? window + SPAN_ALIGN - 1 : b->max_len;
   const int64_t chunks = chunks_bound(b->n_seqs, P->n_rows, units_of(Span{0, span}, unit));
-  if (chunks * n_heads > 0x7fffffff)
+  if (chunks * n_heads > 0x70000000)
     return fail(c, C2H_ERR_UNSUPPORTED, "%lld chunks of %d heads exceed one launch", (long long)chunks, n_heads);
   P->grid = (int)std::min<int64_t>(chunks * P->n_rows, ATTN_WGS);
   *parts = span > unit ? chunks * n_heads : 0;

@@ -460,36 +460,68 @@ __device__ __forceinline__ Cut cut_batch(const int32_t* lens, int n_seqs, int ma
   const int lane = threadIdx.x & 63;
   Cut c{(n_seqs + 63) >> 6, 1, 0, 0, n_seqs};
   if (!split) return c;  // no session is longer than a unit
-  int64_t units = 0;
+  auto units_at = [&](int len) { return session_units<UNIT>(len, max_len, window); };
   if (c.per == 1) {
     c.len = lane < n_seqs ? lens[lane] : 0;
-    units = __builtin_amdgcn_readlane(scan_of_wave(session_units<UNIT>(c.len, max_len, window)), 63);
+    c.units = chunk_units(__builtin_amdgcn_readlane(scan_of_wave(units_at(c.len)), 63), n_rows);
+    c.upto = scan_of_wave(lane < n_seqs ? chunks_of(units_at(c.len), c.units) : 0);
   } else {
-    int mine = 0;  // below 2^31: 1024 sessions of 2^17 units
-    for (int k = 0; k < c.per; ++k) {
-      const int s = lane * c.per + k;
-      mine += s < n_seqs ? session_units<UNIT>(lens[s], max_len, window) : 0;
+    // eight lengths of the lane's at a time, loaded together
+    int v[8];
+    auto load8 = [&](int k) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = lens[min(lane * c.per + k + i, n_seqs - 1)];
+    };
+    auto sum8 = [&](int k, auto of) {
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += k + i < c.per && lane * c.per + k + i < n_seqs ? of(v[i]) : 0;
+      return sum;
+    };
+    int mine = 0, n = 0;  // below 2^31: 1024 sessions of 2^17 units
+    for (int k = 0; k < c.per; k += 8) {
+      load8(k);
+      mine += sum8(k, units_at);
     }
+    int64_t units = 0;
     for (int m = 0; m < 64; ++m) units += __builtin_amdgcn_readlane(mine, m);
-  }
-  c.units = chunk_units(units, n_rows);
-  int n = 0;
-  if (c.per == 1) {
-    n = lane < n_seqs ? chunks_of(session_units<UNIT>(c.len, max_len, window), c.units) : 0;
-  } else {
-    for (int k = 0; k < c.per; ++k) {
-      const int s = lane * c.per + k;
-      n += s < n_seqs ? chunks_of(session_units<UNIT>(lens[s], max_len, window), c.units) : 0;
+    c.units = chunk_units(units, n_rows);
+    for (int k = 0; k < c.per; k += 8) {
+      if (c.per > 8) load8(k);
+      n += sum8(k, [&](int len) { return chunks_of(units_at(len), c.units); });
     }
+    c.upto = scan_of_wave(n);
   }
-  c.upto = scan_of_wave(n);
   c.total = __builtin_amdgcn_readlane(c.upto, 63);
   return c;
 }
 
+// One new token per session: workgroups take chunks in turn, a chunk's steps
+// go round its four waves, and a row of one chunk is written here, others'
+// parts are joined by k_paged_join.
+// Bound by memory where there is much to read: 8 sessions of 32,768 positions,
+// 16/8 heads of 128, f16 in pages of 64 (1,059 MB) 163 us, 6.5 TB/s; 64
+// sessions of 30 to 8,000, 12/2 heads, bf16 (92 MB) 18.6 us, 4.9 TB/s; 128 of
+// up to 4,096, 16/2 heads, e4m3 (161 MB) 40.8 us, 4.0 TB/s.  The matrix units
+// are busy 8 % of that, the VALU 20 to 37 %.  Otherwise by the chain length ->
+// page -> keys: one session of 41 5.2 us, of 4,096 8.2 us.  16 KB a wave and
+// two workgroups to a CU keep 32 MB in flight, more than the memory's latency
+// times its rate; 512 workgroups and 1,024 chunks took 21.2 us where 512
+// chunks took 25.1 and 2,048 24.6 (64 sessions, with the join).
+//
 // The leading arguments arrive in registers at wave start (kernel-argument
 // preload).  shape: log2 of the page size; from bit 4: whether sessions can
 // have several chunks; from bit 5: n_tiles; from bit 14: n_kv_heads.
+// The block P is read where it is used, through its place in the kernel's
+// arguments: kept in registers over the loop, its fields spill.
+struct AttnLead {
+  const int32_t *lens, *table;
+  int64_t table_stride;
+  int max_len, window;
+  uint32_t shape;
+  int n_seqs;
+};
+static_assert(sizeof(AttnLead) % alignof(PagedAttnParams) == 0, "P follows the leading arguments");
 using Args = const __attribute__((address_space(4))) PagedAttnParams*;
 template <int CT, int HD, bool FULL, bool PRECISE, bool STREAM>
 __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 : 2)
@@ -501,10 +533,9 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   __shared__ __align__(16) char lds[A::LDS];
   __shared__ float mul[16], wm[4][16], wl[4][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, j = lane >> 4;
-  // the block behind the leading arguments, read where it is used: kept in
-  // registers over the loop below, its fields spill
   auto fresh = [&]() {
-    Args a = (Args)((const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr() + 40), b;
+    auto* lead = (const __attribute__((address_space(4))) AttnLead*)__builtin_amdgcn_kernarg_segment_ptr();
+    Args a = (Args)(lead + 1), b;
     asm volatile("" : "=s"(b) : "0"(a));
     return b;
   };
@@ -876,7 +907,10 @@ __global__ void __launch_bounds__(256, HD == 256 && (CT == PT_F32 || !FULL) ? 1 
   }
 }
 
-// Joins the chunks of a row: the sums brought to the common maximum.  One
+// Joins the chunks of a row: the sums brought to the common maximum (2.9 us
+// for 16 rows of 32 chunks, 5 us for 768 or 2,048 rows of a few; a join in the
+// first launch, by the row's last workgroup, was slower: 26.7 us in all for 22
+// at 64 sessions).  One
 // workgroup per row; HDP / 4 threads hold the row's elements, and 1024 / HDP
 // groups of them take every so-manieth chunk.
 template <int HDP>

@@ -399,10 +399,12 @@ int c2h_paged_append_dev(c2h_ctx* ctx, const c2h_paged_kv* kv, const c2h_paged_b
  * over the positions j < seq_lens[s] (the last `window` of them where
  * window > 0) of KV head h / (n_heads / n_kv_heads).  q and out are
  * [n_seqs][n_heads] vectors of `type` (F32, F16, BF16), not overlapping.  A
- * session of length 0 gets zeros.  Scores, softmax and sums are 32-bit, the
+ * session of length 0 gets zeros.  What a session holds is to be finite (a
+ * NaN or an infinity there makes its head's rows NaN or infinite); what stands
+ * elsewhere in the pool does not matter.  Scores, softmax and sums are 32-bit, the
  * result is rounded once to `type`; the same call on the same data gives the
- * same bits (how long sessions are split follows from n_seqs, max_len,
- * window and the pool's description alone).
+ * same bits (how long sessions are split follows from the batch's lengths and
+ * the descriptions alone).
  * Work of several workgroups on one row meets in a workspace of the
  * context, which c2h_paged_attn_workspace sizes; it grows, with a wait for
  * the stream, in the first call that needs more than any before. */

@@ -187,6 +187,17 @@ def test_attention_split_sessions(ctx, cache, ty, n):
     check_attention(ctx, [n, 1, 0, 700, n // 2], 14, 2, 64, 16, "hnd", cache, ty, seed=n)
 
 
+@pytest.mark.parametrize("n", [63, 64, 65, 129, 513, 1500])
+@pytest.mark.parametrize("window", [0, 200])
+def test_attention_many_sessions(ctx, n, window):
+    # each lane of a wave looks after one session, a few, more than eight;
+    # some are split, some empty
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 40, n)
+    lens[rng.integers(0, n, 8)] = rng.integers(300, 2500, 8)
+    check_attention(ctx, lens.tolist(), 2, 1, 16, 16, "nhd", H.F32, H.F32, window=window, seed=n)
+
+
 @pytest.mark.parametrize("cache,ty", [(H.F32, H.F32), (H.BF16, H.BF16), (H.F8_E4M3, H.F16)], ids=lambda t: NAMES[t])
 @pytest.mark.parametrize("window", [0, 1111])
 def test_attention_chunks_of_more_pages_than_lanes(ctx, cache, ty, window):
