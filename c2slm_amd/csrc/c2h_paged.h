@@ -23,6 +23,7 @@ constexpr int PAGED_MAX_PAGE = 1024;
 constexpr int PAGED_MAX_LEN = 1 << 23; // chunks are a grid's third index
 constexpr int ATTN_HEADS = 16;         // query heads of a workgroup: columns of the matrix instruction
 constexpr int ATTN_CHUNKS = 1024;      // chunks that a batch is cut into
+constexpr int ATTN_MANY_ROWS = 2048;   // rows from which the join takes several a workgroup
 constexpr int ATTN_WGS = 512;          // workgroups that take them in turn
 
 // The positions [lo, hi) that a session of `len` positions attends, `window`

@@ -972,12 +972,66 @@ __global__ void __launch_bounds__(256) k_paged_join(const int32_t* info, const f
   }
 }
 
+// The same for batches of many rows, most of a few chunks or one: HDP / 4
+// threads to a row, nothing shared between them.  From 2,048 rows (128
+// sessions of e4m3: 43.7 us in all for 45.0; 500 sessions of 20 to 900, 8,000
+// rows: 33.2 for 35.4); at 768 rows of up to 30 chunks the row's one thread
+// group is the slower one (25.0 for 22.1).
+template <int HDP>
+__global__ void __launch_bounds__(256) k_paged_join_rows(const int32_t* info, const float* part_o, const float* part_ml, int rows,
+                                                         PagedAttnParams P) {
+  constexpr int LANES = HDP / 4, ROWS = 256 / LANES, AHEAD = 4;
+  const int row = blockIdx.x * ROWS + threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4, hd = P.kv.head_dim;
+  if (row >= rows || d >= hd) return;
+  const int s = row / P.n_heads, head = row - s * P.n_heads;
+  const int2 where = *reinterpret_cast<const int2*>(info + 2 * s);
+  const int n = where.y;
+  if (n <= 1) return;
+  const int64_t first = (int64_t)where.x * P.n_heads + head;
+  f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f};
+  float m = MINUS_INF, l = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += AHEAD) {
+    float2 x[AHEAD];
+    f32x4 v[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int64_t part = first + (int64_t)min(i0 + k, n - 1) * P.n_heads;
+      x[k] = *reinterpret_cast<const float2*>(part_ml + part * 2);
+      v[k] = *reinterpret_cast<const f32x4*>(part_o + part * hd + d);
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      if (i0 + k >= n) x[k] = make_float2(MINUS_INF, 0.0f), v[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      top = fmaxf(top, x[k].x);
+    }
+    const float mu = finite_max(top), was = weight(m, mu);
+    a *= was;
+    l *= was;
+    m = top;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const float w = weight(x[k].x, mu);
+      a += v[k] * w;
+      l += x[k].y * w;
+    }
+  }
+  // no weight at all: zeros, but the NaN of a bad table stays
+  store4(P.type, P.out.data + s * P.out.token_stride + head * P.out.head_stride + (int64_t)d * (P.type == PT_F32 ? 4 : 2),
+         l == 0.0f ? a * 0.0f : a / l);
+}
+
 template <int CT, int HD, bool FULL, bool PRECISE, bool STREAM>
 void launch_attn_as(const PagedAttnParams& P, hipStream_t st) {
   const uint32_t shape = (uint32_t)P.kv.page_shift | (P.info ? 16u : 0u) | (uint32_t)P.n_tiles << 5 | (uint32_t)P.kv.n_kv_heads << 14;
   hipLaunchKernelGGL((k_paged_attn<CT, HD, FULL, PRECISE, STREAM>), dim3(P.grid), dim3(256), 0, st, P.b.lens, P.b.table,
                      P.b.table_stride, P.b.max_len, P.window, shape, P.b.n_seqs, P);
-  if (P.info)
+  if (!P.info) return;
+  const int rows = P.n_heads * P.b.n_seqs;
+  if (rows >= ATTN_MANY_ROWS)
+    hipLaunchKernelGGL(k_paged_join_rows<HD>, dim3((rows + 1023 / HD) / (1024 / HD)), dim3(256), 0, st, P.info, P.part_o,
+                       P.part_ml, rows, P);
+  else
     hipLaunchKernelGGL(k_paged_join<HD>, dim3(P.n_heads, P.b.n_seqs), dim3(256), 0, st, P.info, P.part_o, P.part_ml, P);
 }
 
