@@ -115,7 +115,7 @@ def attention64(sess, q, scale, window, ty):
     return out, tol + rounding(out, ty)
 
 
-def run_attention(ctx, sess, q, scale, window=0, extra_rows=2, sync=True):
+def run_attention(ctx, sess, q, scale, window=0, extra_rows=2):
     """The kernel's rows on a strided q and an out with rows beyond the batch."""
     kv, batch = sess.cuda()
     n, heads, dim = q.shape
@@ -126,8 +126,7 @@ def run_attention(ctx, sess, q, scale, window=0, extra_rows=2, sync=True):
     torch.cuda.synchronize()
     ctx.paged_attn_dev(kv, batch, ty, heads, scale, H.heads(fused[:, 1:heads + 1, :dim]), H.heads(buf[:n, :heads]),
                        window=window)
-    if sync:
-        ctx.sync()
+    ctx.sync()
     got = buf.cpu()
     assert (got[n:] == 5.0).all() and (got[:n, heads:] == 5.0).all(), "rows behind the batch changed"
     return got[:n, :heads].double()
@@ -196,6 +195,102 @@ def test_attention_many_sessions(ctx, n, window):
     lens = rng.integers(0, 40, n)
     lens[rng.integers(0, n, 8)] = rng.integers(300, 2500, 8)
     check_attention(ctx, lens.tolist(), 2, 1, 16, 16, "nhd", H.F32, H.F32, window=window, seed=n)
+
+
+@pytest.mark.parametrize("dim,cache,ty", [(64, H.F16, H.F16), (80, H.F32, H.BF16), (128, H.BF16, H.F32), (144, H.F16, H.F32),
+                                          (256, H.F8_E4M3, H.BF16)], ids=str)
+def test_attention_join_of_many_rows(ctx, dim, cache, ty):
+    # 2,200 rows: most of one chunk, some of several, empty ones and a bad page
+    rng = np.random.default_rng(dim)
+    lens = rng.integers(0, 30, 1100)
+    lens[[0, 7, 500, 1099]] = [3000, 700, 1111, 2000]
+    check_attention(ctx, lens.tolist(), 2, 1, dim, 16, "hnd", cache, ty, seed=dim)
+    sess = Sessions([int(n) for n in lens], 1, dim, 16, "hnd", cache, dim)
+    sess.table[500, 40] = -1
+    kv, batch = sess.cuda()
+    q = torch.ones(1100, 2, dim).to(TORCH[ty]).cuda()
+    out = torch.full_like(q, 5.0)
+    torch.cuda.synchronize()
+    ctx.paged_attn_dev(kv, batch, ty, 2, 0.01, H.heads(q), H.heads(out))
+    with pytest.raises(H.C2hError):
+        ctx.sync()
+    got = out.cpu()
+    assert torch.isnan(got[500]).all() and torch.isfinite(got[torch.arange(1100) != 500]).all()
+
+
+def strided_pool(sess, how):
+    """The session's pools laid out otherwise on the GPU: (k, v) views."""
+    k, v = sess.pools
+    if how == "side by side":  # a page's keys, then its values
+        both = torch.stack([k.view(torch.int8) if sess.cache == H.F8_E4M3 else k, v.view(torch.int8) if sess.cache == H.F8_E4M3 else v], 1).cuda()
+        if sess.cache == H.F8_E4M3:
+            both = both.view(TORCH[sess.cache])
+        return both, both[:, 0], both[:, 1]
+    if how == "heads outermost":
+        out = [p.permute(2, 0, 1, 3).contiguous().cuda().permute(1, 2, 0, 3) for p in sess.pools]
+        return out, out[0], out[1]
+    wide = [torch.zeros((p.shape[0], p.shape[1] + 1, p.shape[2] + 2, p.shape[3] + 16), dtype=p.dtype) for p in sess.pools]
+    for w, p in zip(wide, sess.pools):  # gaps after elements, heads, tokens
+        w[:, :-1, :-2, :-16] = p
+    wide = [w.cuda() for w in wide]
+    return wide, *(w[:, :-1, :-2, :-16] for w in wide)
+
+
+@pytest.mark.parametrize("how", ["side by side", "heads outermost", "gaps"])
+@pytest.mark.parametrize("cache", [H.F32, H.BF16], ids=lambda t: NAMES[t])
+def test_pools_of_other_strides(ctx, how, cache):
+    # append three tokens a session, then attend with one query for all sessions
+    lens = [3, 40, 300, 17]
+    sess = Sessions(lens, 2, 64, 16, "nhd", cache, 3)
+    g = torch.Generator().manual_seed(4)
+    kn, vn = torch.randn(12, 2, 64, generator=g), torch.randn(12, 2, 64, generator=g)
+    keep, k, v = strided_pool(sess, how)
+    sess.cuda()
+    kv, batch = H.paged_kv(k, v, cache), H.paged_batch(sess.table_d, sess.lens_d, max(lens))
+    start = torch.tensor([0, 3, 6, 9, 12], dtype=torch.int32).cuda()
+    kd, vd = kn.cuda(), vn.cuda()
+    q = torch.randn(1, 4, 64, generator=g).cuda()
+    out = torch.zeros(4, 4, 64, device="cuda")
+    torch.cuda.synchronize()
+    ctx.paged_append_dev(kv, batch, H.F32, 12, H.heads(kd), H.heads(vd), token_start=start)
+    ctx.paged_attn_dev(kv, batch, H.F32, 4, 0.125, H.Heads(q.data_ptr(), 0, 64), H.heads(out))
+    ctx.sync()
+    for s, n in enumerate(lens):
+        for i, x in enumerate((kn, vn)):
+            sess.rows[s][i][n - 3:] = x[3 * s:3 * s + 3].to(TORCH[cache]).double()
+    want, tol = attention64(sess, q.cpu().expand(4, 4, 64), 0.125, 0, H.F32)
+    assert ((out.cpu().double() - want).abs() <= tol).all()
+    if how == "gaps":
+        assert all((w[:, -1:] == 0).all() and (w[:, :, -2:] == 0).all() and (w[..., -16:] == 0).all() for w in keep)
+
+
+def test_offsets_beyond_32_bits(ctx):
+    # a pool of 6 GiB each of keys and values: pages at its start and its end
+    pages = (6 << 30) // (16 * 8 * 128 * 2)
+    pool = [torch.empty((pages, 16, 8, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    used = [pages - 1, 0, pages - 2, pages // 2, pages // 3 * 2]
+    lens = [70]
+    sess = Sessions(lens, 8, 128, 16, "nhd", H.BF16, 8, spare=0)
+    rank = {int(p): u for p, u in zip(sess.table[0, :5], used)}
+    for i in range(2):
+        for p, u in rank.items():
+            pool[i][u] = sess.pools[i][p].cuda()
+    table = torch.tensor([used], dtype=torch.int32).cuda()
+    lens_d = torch.tensor(lens, dtype=torch.int32).cuda()
+    kv, batch = H.paged_kv(pool[0], pool[1], H.BF16), H.paged_batch(table, lens_d, 80)
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(1, 16, 128, generator=g).bfloat16()
+    x = torch.randn(1, 16, 128, generator=g).bfloat16().cuda()  # the 70th token: page 4, slot 5
+    qd, out = q.cuda(), torch.zeros(1, 16, 128, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    ctx.paged_append_dev(kv, batch, H.BF16, 1, H.heads(x[:, :8]), H.heads(x[:, 8:]))
+    ctx.paged_attn_dev(kv, batch, H.BF16, 16, 0.1, H.heads(qd), H.heads(out))
+    ctx.sync()
+    for i in range(2):
+        sess.rows[0][i][69] = x[0, 8 * i:8 * i + 8].cpu().double()
+        assert torch.equal(pool[i][used[4], 5], x[0, 8 * i:8 * i + 8])
+    want, tol = attention64(sess, q, 0.1, 0, H.BF16)
+    assert ((out.cpu().double() - want).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("cache,ty", [(H.F32, H.F32), (H.BF16, H.BF16), (H.F8_E4M3, H.F16)], ids=lambda t: NAMES[t])
