@@ -2681,6 +2681,8 @@ int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int 
   if (n_heads < 1 || n_heads > 4096 || n_heads % kv->n_kv_heads)
     return fail(c, C2H_ERR_INVALID, "%d query heads over %d KV heads", n_heads, kv->n_kv_heads);
   if (window < 0) return fail(c, C2H_ERR_INVALID, "window %d", window);
+  if ((int64_t)b->n_seqs * n_heads > MAX_SESSION_HEADS)
+    return fail(c, C2H_ERR_UNSUPPORTED, "%d sessions of %d heads: up to %d rows", b->n_seqs, n_heads, MAX_SESSION_HEADS);
   P->n_heads = n_heads;
   P->group = n_heads / kv->n_kv_heads;
   P->n_tiles = (P->group + ATTN_HEADS - 1) / ATTN_HEADS;
@@ -2741,6 +2743,7 @@ int c2h_rope_init(const c2h_rope_desc* d, c2h_rope* r) {
 int c2h_rope_dev(c2h_ctx* c, const c2h_rope* rope, int32_t type, const c2h_heads* x, const int32_t* positions,
                  int32_t n_tokens, int32_t n_heads, int32_t head_dim, const c2h_heads* y) {
   if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
+  if (n_tokens > MAX_TOKENS) return fail(c, C2H_ERR_UNSUPPORTED, "%d tokens: up to %d", n_tokens, MAX_TOKENS);
   if (n_tokens < 0 || n_heads < 1 || n_heads > 4096) return fail(c, C2H_ERR_INVALID, "%d tokens of %d heads", n_tokens, n_heads);
   if (head_dim < 8 || head_dim > C2H_ROPE_MAX_DIM || head_dim % 8)
     return fail(c, C2H_ERR_UNSUPPORTED, "head_dim %d: a multiple of 8 up to %d", head_dim, C2H_ROPE_MAX_DIM);
@@ -2772,6 +2775,7 @@ int c2h_paged_append_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_bat
   int rc = check_paged(c, kv, b);
   if (rc) return rc;
   if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
+  if (n_tokens > MAX_TOKENS) return fail(c, C2H_ERR_UNSUPPORTED, "%d tokens: up to %d", n_tokens, MAX_TOKENS);
   if (n_tokens < 0 || (!token_start && n_tokens != b->n_seqs))
     return fail(c, C2H_ERR_INVALID, "%d tokens for %d sessions without token_start", n_tokens, b->n_seqs);
   if (rope && (rc = check_rope(c, rope, kv->head_dim))) return rc;
@@ -2867,6 +2871,7 @@ int c2h_rmsnorm_q8k_dev(c2h_ctx* c, int32_t type, const void* x, int64_t x_strid
                         int64_t sum_stride, void* q8k_out, float* y_out, int64_t y_stride) {
   if (!act_type(type)) return fail(c, C2H_ERR_UNSUPPORTED, "type %d", type);
   if (n_rows < 0) return fail(c, C2H_ERR_INVALID, "%d rows", n_rows);
+  if (n_rows > MAX_NORM_ROWS) return fail(c, C2H_ERR_UNSUPPORTED, "%d rows: up to %d", n_rows, MAX_NORM_ROWS);
   if (cols < 256 || cols > 16384) return fail(c, C2H_ERR_UNSUPPORTED, "%d columns: 256 to 16384", cols);
   if (n_rows > 0 && (!x || !w || !q8k_out || (residual != nullptr) != (sum_out != nullptr)))
     return fail(c, C2H_ERR_INVALID, "x, w and q8k_out are required, residual and sum_out come together");

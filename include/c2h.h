@@ -327,7 +327,7 @@ int c2h_rope_init(const c2h_rope_desc* desc, c2h_rope* rope);
 
 /* y = x rotated, for n_tokens tokens of n_heads heads of head_dim elements
  * (a multiple of 8 up to 256, at least rot_dim) of type F32, F16 or BF16;
- * token t stands at positions[t] (device, int32).  32-bit arithmetic, one
+ * token t stands at positions[t] (device, int32); up to 2^24 - 1 tokens.  32-bit arithmetic, one
  * rounding to the type.  y may be x itself (same pointer and strides);
  * otherwise they must not overlap. */
 int c2h_rope_dev(c2h_ctx* ctx, const c2h_rope* rope, int32_t type, const c2h_heads* x, const int32_t* positions,
@@ -387,7 +387,7 @@ typedef struct c2h_paged_batch {
  * none), n_heads vectors per token, goes to q_out, rotated, in `type`;
  * q_out may be q (same pointer and strides).  Tokens from
  * token_start[n_seqs] on and those of sessions of length 0 are no tokens:
- * their q_out rows are left as they were.  Pages shared between sessions
+ * their q_out rows are left as they were.  Up to 2^24 - 1 tokens a call.  Pages shared between sessions
  * are read only: no two tokens of a call may come to stand in one slot. */
 int c2h_paged_append_dev(c2h_ctx* ctx, const c2h_paged_kv* kv, const c2h_paged_batch* batch,
                          const int32_t* token_start, int32_t n_tokens, const c2h_rope* rope, int32_t type,
@@ -398,7 +398,8 @@ int c2h_paged_append_dev(c2h_ctx* ctx, const c2h_paged_kv* kv, const c2h_paged_b
  *   out = sum_j p_j v_j,  p = softmax_j(scale * q . k_j)
  * over the positions j < seq_lens[s] (the last `window` of them where
  * window > 0) of KV head h / (n_heads / n_kv_heads).  q and out are
- * [n_seqs][n_heads] vectors of `type` (F32, F16, BF16), not overlapping.  A
+ * [n_seqs][n_heads] vectors of `type` (F32, F16, BF16), up to 2^24 - 1 of them,
+ * not overlapping.  A
  * session of length 0 gets zeros.  What a session holds is to be finite (a
  * NaN or an infinity there makes its head's rows NaN or infinite); what stands
  * elsewhere in the pool does not matter.  Scores, softmax and sums are 32-bit, the
@@ -417,7 +418,7 @@ int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* batc
                              size_t* bytes);
 
 /* RMSNorm with the residual's addition and Q8_K rows as its output: for each
- * of n_rows rows of cols elements (256 .. 16384) of `type` (F32, F16, BF16)
+ * of n_rows (up to 2^22 - 1) rows of cols elements (256 .. 16384) of `type` (F32, F16, BF16)
  *   s = x + residual (rounded to the type and stored to sum_out; s = x where
  *       residual is NULL),
  *   y = (s * f32(1 / sqrt(mean(s^2) + eps))) * w,

@@ -135,6 +135,36 @@ def test_append_and_rope_arguments_refused():
     refused(rope(), INVALID, "no context")
 
 
+def test_more_than_a_launch_refused():
+    """Work-items of a launch are counted in 32 bits."""
+    L, r, row = H.lib(), H.rope(64, 1e6), heads(token_stride=1024, head_stride=64)
+    # one row of all sessions' queries; outputs of 2^18 elements a session
+    q, out = heads(token_stride=0), heads(token_stride=1 << 18)
+
+    def rope(n):
+        return L.c2h_rope_dev(None, r, H.F32, row, A, n, 4, 64, row)
+
+    def app(n):
+        return L.c2h_paged_append_dev(None, kv(), batch(), A, n, None, H.F32, row, row, 0, None, None)
+
+    def attn(n_seqs, n_heads):
+        return L.c2h_paged_attn_dev(None, kv(), batch(n_seqs=n_seqs), H.F32, n_heads, 0.1, 0, q, out)
+
+    def norm(n):
+        return L.c2h_rmsnorm_q8k_dev(None, H.F32, A, 256, None, 0, A, 1e-6, n, 256, None, 0, A, None, 0)
+
+    for call, most in ((rope, 2 ** 24 - 1), (app, 2 ** 24 - 1), (norm, 2 ** 22 - 1)):
+        refused(call(most), INVALID, "no context")
+        for n in (most + 1, 2 ** 31 - 1):
+            refused(call(n), UNSUPPORTED, "up to %d" % most)
+    refused(attn(65535, 256), INVALID, "no context")
+    refused(attn(65535, 258), UNSUPPORTED, "65535 sessions of 258 heads")
+    refused(attn(4096, 4096), UNSUPPORTED, "4096 sessions of 4096 heads")
+    n = C.c_size_t(7)
+    refused(L.c2h_paged_attn_workspace(kv(), batch(n_seqs=65535), 4096, 0, C.byref(n)), UNSUPPORTED, "sessions")
+    assert n.value == 0
+
+
 def test_norm_arguments_refused():
     L = H.lib()
 
