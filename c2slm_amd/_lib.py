@@ -392,12 +392,12 @@ class Ctx:
 
     # ---- operators for many sessions (device memory; asynchronous: sync() waits)
     #
-    # Tensors are objects with data_ptr(), stride() and shape (torch's), on
-    # the context's GPU and complete; they must live until the work is done.
+    # Tensors are torch's (or objects with the methods used here), on the
+    # context's GPU and complete; they must live until the work is done.
     def rope_dev(self, rope: Rope, ggml_type: int, x: Heads, positions, n_tokens: int, n_heads: int, head_dim: int,
                  y: Heads):
         """y = x rotated to positions (c2h_rope_dev)."""
-        rc = _lib.c2h_rope_dev(self.h, rope, ggml_type, x, _dp(positions), n_tokens, n_heads, head_dim, y)
+        rc = _lib.c2h_rope_dev(self.h, rope, ggml_type, x, _ip(positions), n_tokens, n_heads, head_dim, y)
         if rc:
             self._chk(rc)
 
@@ -406,7 +406,7 @@ class Ctx:
                          n_heads: int = 0):
         """Keys and values of new tokens into their pages, K rotated, and the
         queries rotated to q_out (c2h_paged_append_dev)."""
-        rc = _lib.c2h_paged_append_dev(self.h, kv, batch, _dp(token_start), n_tokens, rope, ggml_type, k, v, n_heads, q,
+        rc = _lib.c2h_paged_append_dev(self.h, kv, batch, _ip(token_start), n_tokens, rope, ggml_type, k, v, n_heads, q,
                                        q_out)
         if rc:
             self._chk(rc)
@@ -422,17 +422,40 @@ class Ctx:
         """Rows of x (plus residual, to sum_out) normalised, times w, to Q8_K
         rows and, where y is given, floats (c2h_rmsnorm_q8k_dev)."""
         n, cols = x.shape
-        rp, rs = (residual.data_ptr(), residual.stride(0)) if residual is not None else (None, 0)
-        sp, ss = (sum_out.data_ptr(), sum_out.stride(0)) if sum_out is not None else (None, 0)
-        yp, ys = (y.data_ptr(), y.stride(0)) if y is not None else (None, 0)
-        rc = _lib.c2h_rmsnorm_q8k_dev(self.h, ggml_type, x.data_ptr(), x.stride(0), rp, rs, w.data_ptr(), eps, n, cols, sp,
-                                      ss, q8k.data_ptr(), yp, ys)
+        xp, xs = _rows(x, n, cols)
+        rp, rs = _rows(residual, n, cols)
+        sp, ss = _rows(sum_out, n, cols)
+        yp, ys = _rows(y, n, cols)
+        if w.numel() != cols or not w.is_contiguous() or q8k.nbytes < n * (cols // 256) * 292 or not q8k.is_contiguous():
+            raise ValueError("rmsnorm_q8k_dev() takes a weight per column and 292 bytes per 256 of them in each row")
+        rc = _lib.c2h_rmsnorm_q8k_dev(self.h, ggml_type, xp, xs, rp, rs, w.data_ptr(), eps, n, cols, sp, ss, q8k.data_ptr(),
+                                      yp, ys)
         if rc:
             self._chk(rc)
 
 
 def _dp(t):
     return None if t is None else t.data_ptr()
+
+
+def _ip(t):
+    """Positions and the like: int32, one after another."""
+    if t is None:
+        return None
+    if t.element_size() != 4 or not t.is_contiguous():
+        raise ValueError("positions, lengths and starts are contiguous int32")
+    return t.data_ptr()
+
+
+def _rows(t, n, cols):
+    """Address and stride of the (first) n rows of a tensor of cols columns."""
+    if t is None:
+        return None, 0
+    stride, one = t.stride()
+    rows, width = t.shape
+    if one != 1 or rows < n or width != cols:
+        raise ValueError("as many rows and columns as x, their elements contiguous")
+    return t.data_ptr(), stride
 
 
 def heads(t) -> Heads:
@@ -474,8 +497,10 @@ def paged_batch(block_table, seq_lens, max_len: int) -> PagedBatch:
     [sessions] on the GPU, and a bound of the lengths."""
     if block_table.ndim != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0]:
         raise ValueError("paged_batch() takes a table [sessions, pages] and as many lengths")
+    if block_table.element_size() != 4:
+        raise ValueError("paged_batch() takes int32 tables")
     return PagedBatch(block_table.data_ptr(), block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
-                      seq_lens.data_ptr(), seq_lens.shape[0], max_len)
+                      _ip(seq_lens), seq_lens.shape[0], max_len)
 
 
 def paged_attn_workspace(kv: PagedKV, batch: PagedBatch, n_heads: int, window: int = 0) -> int:

@@ -2845,7 +2845,11 @@ int c2h_paged_attn_dev(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch
     c->paged_ws = nullptr;
     c->paged_ws_bytes = 0;
     void* p = nullptr;
-    HIPCHK(c, hipMalloc(&p, bytes));
+    const hipError_t e = hipMalloc(&p, bytes);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();  // or the next call's launch would be told of it
+      return fail(c, C2H_ERR_HIP, "no workspace of %zu bytes: %s", bytes, hipGetErrorString(e));
+    }
     c->paged_ws = reinterpret_cast<float*>(p);
     c->paged_ws_bytes = bytes;
   }

@@ -346,3 +346,39 @@ def test_python_views_refused():
         H.rope(64, 1e6, freq_factors=np.ones(31))
     p = H.paged_kv(T((4, 2, 16, 64), (2048, 1024, 64, 1)), T((4, 2, 16, 64), (2048, 1024, 64, 1)), H.BF16, order="hnd")
     assert (p.page_size, p.n_kv_heads, p.token_stride, p.head_stride) == (16, 2, 64, 1024)
+
+
+def test_python_tensors_of_other_shapes_and_types_refused():
+    """What Python's calls take by address they check first: 64-bit indexes
+    (torch's default) or a column of a tensor would be read as other numbers,
+    rows of another shape beyond their end."""
+    torch = pytest.importorskip("torch")
+    ctx = object.__new__(H.Ctx)
+    ctx.h = None
+    lens, table = torch.ones(2, dtype=torch.int32), torch.ones(2, 4, dtype=torch.int32)
+    assert H.paged_batch(table, lens, 64).n_seqs == 2
+    for t, n in ((table.long(), lens), (table, lens.long()), (table, table[:, 0])):
+        with pytest.raises(ValueError):
+            H.paged_batch(t, n, 64)
+    rope, x = H.rope(64, 1e6), heads()
+    kv_, batch_ = kv(), batch()
+    for bad in (torch.arange(3), torch.ones(3, 2, dtype=torch.int32)[:, 0]):
+        with pytest.raises(ValueError):
+            ctx.rope_dev(rope, H.F32, x, bad, 3, 4, 64, x)
+        with pytest.raises(ValueError):
+            ctx.paged_append_dev(kv_, batch_, H.F32, 3, x, x, token_start=bad)
+    r, w, q8k = torch.ones(3, 512), torch.ones(512), torch.ones(3, 2, 292, dtype=torch.uint8)
+
+    def norm(x=r, w=w, q8k=q8k, **more):
+        with pytest.raises(ValueError):
+            ctx.rmsnorm_q8k_dev(H.F32, x, w, 1e-6, q8k, **more)
+
+    norm(x=torch.ones(512, 3).T)
+    norm(w=w[:256])
+    norm(w=torch.ones(1024)[::2])
+    norm(q8k=q8k[:2])
+    norm(q8k=torch.ones(3, 2, 584, dtype=torch.uint8)[:, :, :292])
+    for bad in (r[:2], r[:, :256], torch.ones(512, 3).T, torch.ones(3, 1024)[:, ::2]):
+        norm(residual=bad, sum_out=r)
+        norm(residual=r, sum_out=bad)
+        norm(y=bad)
