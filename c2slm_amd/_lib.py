@@ -488,6 +488,9 @@ def paged_kv(k, v, ggml_type: int, order: str = "nhd", k_scale=None, v_scale=Non
     if k.shape != v.shape or k.stride() != v.stride() or k.ndim != 4 or k.stride(3) != 1:
         raise ValueError("paged_kv() takes two pools of four dimensions, of equal shapes and strides")
     t, h = (1, 2) if order == "nhd" else (2, 1)
+    for scale in (k_scale, v_scale):
+        if scale is not None and (scale.element_size() != 4 or not scale.is_contiguous() or scale.numel() != k.shape[h]):
+            raise ValueError("paged_kv() takes a 32-bit scale per KV head")
     return PagedKV(k.data_ptr(), v.data_ptr(), ggml_type, k.shape[0], k.shape[t], k.shape[h], k.shape[3], 0, k.stride(0),
                    k.stride(t), k.stride(h), _dp(k_scale), _dp(v_scale))
 

@@ -360,6 +360,13 @@ def test_python_tensors_of_other_shapes_and_types_refused():
     for t, n in ((table.long(), lens), (table, lens.long()), (table, table[:, 0])):
         with pytest.raises(ValueError):
             H.paged_batch(t, n, 64)
+    pool = torch.ones(4, 16, 2, 64, dtype=torch.uint8)
+    assert H.paged_kv(pool, pool, H.F8_E4M3, k_scale=torch.ones(2)).k_scale
+    for bad in (torch.ones(2, dtype=torch.bfloat16), torch.ones(1), torch.ones(16), torch.ones(2, 2)[:, 0]):
+        with pytest.raises(ValueError):
+            H.paged_kv(pool, pool, H.F8_E4M3, k_scale=bad)
+        with pytest.raises(ValueError):
+            H.paged_kv(pool, pool, H.F8_E4M3, v_scale=bad)
     rope, x = H.rope(64, 1e6), heads()
     kv_, batch_ = kv(), batch()
     for bad in (torch.arange(3), torch.ones(3, 2, dtype=torch.int32)[:, 0]):
