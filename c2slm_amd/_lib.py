@@ -18,6 +18,7 @@ C2H_OK = 0
 NOALLOC_MAX_COLS = 16384  # C2H_NOALLOC_MAX_COLS
 F32, Q5_0, Q8_0, Q4_K, Q6_K = 0, 6, 8, 12, 14
 F16, BF16, F8_E4M3 = 1, 30, 100  # activations and paged caches
+ELEMENT = {F32: "float32", F16: "float16", BF16: "bfloat16"}  # the tensors that hold activations
 ROPE_LAYOUT = dict(half=0, interleaved=1)  # C2H_ROPE_*
 ROPE_MAX_DIM = 256
 
@@ -422,16 +423,32 @@ class Ctx:
         """Rows of x (plus residual, to sum_out) normalised, times w, to Q8_K
         rows and, where y is given, floats (c2h_rmsnorm_q8k_dev)."""
         n, cols = x.shape
-        xp, xs = _rows(x, n, cols)
-        rp, rs = _rows(residual, n, cols)
-        sp, ss = _rows(sum_out, n, cols)
-        yp, ys = _rows(y, n, cols)
+        xs, one = x.stride()
+        own = x.dtype
+        if one != 1 or _KIND[own] != ELEMENT.get(ggml_type):
+            raise ValueError("rmsnorm_q8k_dev() takes rows of the call's type, their elements contiguous")
+        if _KIND[w.dtype] != "float32" or (y is not None and _KIND[y.dtype] != "float32"):
+            raise ValueError("rmsnorm_q8k_dev() takes w and y of float32")
+        rp, rs = _rows(residual, n, cols, own) if residual is not None else (None, 0)
+        sp, ss = _rows(sum_out, n, cols, own) if sum_out is not None else (None, 0)
+        yp, ys = _rows(y, n, cols, y.dtype) if y is not None else (None, 0)
         if w.numel() != cols or not w.is_contiguous() or q8k.nbytes < n * (cols // 256) * 292 or not q8k.is_contiguous():
             raise ValueError("rmsnorm_q8k_dev() takes a weight per column and 292 bytes per 256 of them in each row")
-        rc = _lib.c2h_rmsnorm_q8k_dev(self.h, ggml_type, xp, xs, rp, rs, w.data_ptr(), eps, n, cols, sp, ss, q8k.data_ptr(),
-                                      yp, ys)
+        rc = _lib.c2h_rmsnorm_q8k_dev(self.h, ggml_type, x.data_ptr(), xs, rp, rs, w.data_ptr(), eps, n, cols, sp, ss,
+                                      q8k.data_ptr(), yp, ys)
         if rc:
             self._chk(rc)
+
+
+class _Kinds(dict):
+    """Name of an element type ("float32") by a tensor's dtype."""
+
+    def __missing__(self, dtype):
+        self[dtype] = name = str(dtype).rpartition(".")[2]
+        return name
+
+
+_KIND = _Kinds()
 
 
 def _dp(t):
@@ -447,14 +464,12 @@ def _ip(t):
     return t.data_ptr()
 
 
-def _rows(t, n, cols):
+def _rows(t, n, cols, dtype):
     """Address and stride of the (first) n rows of a tensor of cols columns."""
-    if t is None:
-        return None, 0
     stride, one = t.stride()
     rows, width = t.shape
-    if one != 1 or rows < n or width != cols:
-        raise ValueError("as many rows and columns as x, their elements contiguous")
+    if one != 1 or rows < n or width != cols or t.dtype is not dtype:
+        raise ValueError("rows and columns as x has them, of its type, their elements contiguous")
     return t.data_ptr(), stride
 
 

@@ -389,3 +389,30 @@ def test_python_tensors_of_other_shapes_and_types_refused():
         norm(residual=bad, sum_out=r)
         norm(residual=r, sum_out=bad)
         norm(y=bad)
+
+
+def host_ctx():
+    """A context that no call reaches: every call here is refused before."""
+    ctx = object.__new__(H.Ctx)
+    ctx.h = None
+    return ctx
+
+
+def test_norm_tensors_of_other_element_types_refused():
+    """A weight, row or output of fewer bytes an element than the kernel takes
+    would be read or written beyond its end."""
+    torch = pytest.importorskip("torch")
+    ctx, q8k = host_ctx(), torch.ones(3, 2, 292, dtype=torch.uint8)
+    types = {H.F32: torch.float32, H.F16: torch.float16, H.BF16: torch.bfloat16}
+    H.lib()
+    for ty, own in types.items():
+        good = dict(x=torch.ones(3, 512, dtype=own), w=torch.ones(512), residual=torch.ones(3, 512, dtype=own),
+                    sum_out=torch.ones(3, 512, dtype=own), y=torch.ones(3, 512))
+        for name in good:
+            mine = torch.float32 if name in ("w", "y") else own
+            for other in (torch.float32, torch.float16, torch.bfloat16, torch.float64, torch.int32):
+                if other != mine:
+                    with pytest.raises(ValueError):
+                        ctx.rmsnorm_q8k_dev(ty, eps=1e-6, q8k=q8k, **dict(good, **{name: good[name].to(other)}))
+    with pytest.raises(ValueError):
+        ctx.rmsnorm_q8k_dev(H.F8_E4M3, torch.ones(3, 512), torch.ones(512), 1e-6, q8k)
