@@ -398,7 +398,8 @@ class Ctx:
     def rope_dev(self, rope: Rope, ggml_type: int, x: Heads, positions, n_tokens: int, n_heads: int, head_dim: int,
                  y: Heads):
         """y = x rotated to positions (c2h_rope_dev)."""
-        rc = _lib.c2h_rope_dev(self.h, rope, ggml_type, x, _ip(positions), n_tokens, n_heads, head_dim, y)
+        at = None if positions is None else _ip(positions, n_tokens)
+        rc = _lib.c2h_rope_dev(self.h, rope, ggml_type, x, at, n_tokens, n_heads, head_dim, y)
         if rc:
             self._chk(rc)
 
@@ -407,8 +408,8 @@ class Ctx:
                          n_heads: int = 0):
         """Keys and values of new tokens into their pages, K rotated, and the
         queries rotated to q_out (c2h_paged_append_dev)."""
-        rc = _lib.c2h_paged_append_dev(self.h, kv, batch, _ip(token_start), n_tokens, rope, ggml_type, k, v, n_heads, q,
-                                       q_out)
+        start = None if token_start is None else _ip(token_start, batch.n_seqs + 1)
+        rc = _lib.c2h_paged_append_dev(self.h, kv, batch, start, n_tokens, rope, ggml_type, k, v, n_heads, q, q_out)
         if rc:
             self._chk(rc)
 
@@ -455,12 +456,10 @@ def _dp(t):
     return None if t is None else t.data_ptr()
 
 
-def _ip(t):
-    """Positions and the like: int32, one after another."""
-    if t is None:
-        return None
-    if t.element_size() != 4 or not t.is_contiguous():
-        raise ValueError("positions, lengths and starts are contiguous int32")
+def _ip(t, n):
+    """Address of n positions or the like: int32, one after another."""
+    if _KIND[t.dtype] != "int32" or t.numel() < n or not t.is_contiguous():
+        raise ValueError("positions, lengths and starts are contiguous int32: one per token or session, starts one more")
     return t.data_ptr()
 
 
@@ -515,10 +514,10 @@ def paged_batch(block_table, seq_lens, max_len: int) -> PagedBatch:
     [sessions] on the GPU, and a bound of the lengths."""
     if block_table.ndim != 2 or block_table.stride(1) != 1 or block_table.shape[0] != seq_lens.shape[0]:
         raise ValueError("paged_batch() takes a table [sessions, pages] and as many lengths")
-    if block_table.element_size() != 4:
+    if _KIND[block_table.dtype] != "int32":
         raise ValueError("paged_batch() takes int32 tables")
     return PagedBatch(block_table.data_ptr(), block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
-                      _ip(seq_lens), seq_lens.shape[0], max_len)
+                      _ip(seq_lens, block_table.shape[0]), seq_lens.shape[0], max_len)
 
 
 def paged_attn_workspace(kv: PagedKV, batch: PagedBatch, n_heads: int, window: int = 0) -> int:

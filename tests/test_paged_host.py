@@ -416,3 +416,27 @@ def test_norm_tensors_of_other_element_types_refused():
                         ctx.rmsnorm_q8k_dev(ty, eps=1e-6, q8k=q8k, **dict(good, **{name: good[name].to(other)}))
     with pytest.raises(ValueError):
         ctx.rmsnorm_q8k_dev(H.F8_E4M3, torch.ones(3, 512), torch.ones(512), 1e-6, q8k)
+
+
+def test_fewer_indexes_than_the_call_reads_refused():
+    """Positions one per token, starts one more than sessions, integers of 32
+    bits: floats would be read as their bit patterns, and with the last start
+    missing the last session's tokens would go to another one's slots."""
+    torch = pytest.importorskip("torch")
+    ctx, rope, x = host_ctx(), H.rope(64, 1e6), heads()
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
+    for bad in (i32(1), i32(0), torch.zeros(3), i32(3).view(torch.float32), torch.zeros(6, dtype=torch.int16)):
+        with pytest.raises(ValueError):
+            ctx.rope_dev(rope, H.F32, x, bad, 3, 4, 64, x)
+    for bad in (i32(3), i32(1), torch.zeros(4), torch.zeros(8, dtype=torch.int16)):
+        with pytest.raises(ValueError):
+            ctx.paged_append_dev(kv(), batch(), H.F32, 3, x, x, token_start=bad)
+    table, lens = torch.ones(2, 4, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    for t, n in ((table.float(), lens), (table, lens.float()), (table.view(torch.float32), lens)):
+        with pytest.raises(ValueError):
+            H.paged_batch(t, n, 64)
+    # more than the call reads is fine; without a context the library refuses it
+    for call in (lambda: ctx.rope_dev(rope, H.F32, x, i32(9), 3, 4, 64, x),
+                 lambda: ctx.paged_append_dev(kv(), batch(), H.F32, 3, x, x, token_start=i32(9))):
+        with pytest.raises(H.C2hError, match="no context"):
+            call()
