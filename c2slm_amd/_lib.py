@@ -19,6 +19,7 @@ NOALLOC_MAX_COLS = 16384  # C2H_NOALLOC_MAX_COLS
 F32, Q5_0, Q8_0, Q4_K, Q6_K = 0, 6, 8, 12, 14
 F16, BF16, F8_E4M3 = 1, 30, 100  # activations and paged caches
 ELEMENT = {F32: "float32", F16: "float16", BF16: "bfloat16"}  # the tensors that hold activations
+POOL_ELEMENTS = {**{t: (e,) for t, e in ELEMENT.items()}, F8_E4M3: ("float8_e4m3fn", "uint8", "int8")}
 ROPE_LAYOUT = dict(half=0, interleaved=1)  # C2H_ROPE_*
 ROPE_MAX_DIM = 256
 
@@ -501,10 +502,15 @@ def paged_kv(k, v, ggml_type: int, order: str = "nhd", k_scale=None, v_scale=Non
     ("hnd") of equal strides; k_scale and v_scale: kv_heads floats on the GPU."""
     if k.shape != v.shape or k.stride() != v.stride() or k.ndim != 4 or k.stride(3) != 1:
         raise ValueError("paged_kv() takes two pools of four dimensions, of equal shapes and strides")
+    for pool in (k, v):
+        if hasattr(pool, "dtype") and _KIND[pool.dtype] not in POOL_ELEMENTS.get(ggml_type, ()):
+            raise ValueError("paged_kv() takes pools of the type it is told (F8_E4M3: float8_e4m3fn, or its bits as 8-bit integers)")
+    if order not in ("nhd", "hnd"):
+        raise ValueError("paged_kv(): order is nhd or hnd")
     t, h = (1, 2) if order == "nhd" else (2, 1)
     for scale in (k_scale, v_scale):
-        if scale is not None and (scale.element_size() != 4 or not scale.is_contiguous() or scale.numel() != k.shape[h]):
-            raise ValueError("paged_kv() takes a 32-bit scale per KV head")
+        if scale is not None and (_KIND[scale.dtype] != "float32" or not scale.is_contiguous() or scale.numel() != k.shape[h]):
+            raise ValueError("paged_kv() takes a float32 scale per KV head")
     return PagedKV(k.data_ptr(), v.data_ptr(), ggml_type, k.shape[0], k.shape[t], k.shape[h], k.shape[3], 0, k.stride(0),
                    k.stride(t), k.stride(h), _dp(k_scale), _dp(v_scale))
 

@@ -440,3 +440,35 @@ def test_fewer_indexes_than_the_call_reads_refused():
                  lambda: ctx.paged_append_dev(kv(), batch(), H.F32, 3, x, x, token_start=i32(9))):
         with pytest.raises(H.C2hError, match="no context"):
             call()
+
+
+def test_pools_of_another_element_type_or_order_refused():
+    """A 16-bit pool read as 32-bit ends halfway; an order that is not one of
+    the two was taken for the second."""
+    torch = pytest.importorskip("torch")
+    H.lib()
+    types = {H.F32: torch.float32, H.F16: torch.float16, H.BF16: torch.bfloat16, H.F8_E4M3: torch.float8_e4m3fn}
+    pools = [torch.zeros(4, 16, 2, 64, dtype=torch.uint8).to(t) for t in types.values()]
+    pools += [torch.zeros(4, 16, 2, 64).to(t) for t in (torch.float64, torch.int32, torch.int16, torch.float8_e5m2,
+                                                        torch.float8_e4m3fnuz)]
+    for ty, own in types.items():
+        good = torch.zeros(4, 16, 2, 64, dtype=own)
+        assert H.paged_kv(good, good, ty).type == ty
+        for other in pools:
+            if other.dtype != own:
+                for k, v in ((other, other), (good, other), (other, good)):
+                    with pytest.raises(ValueError):
+                        H.paged_kv(k, v, ty)
+    for bits in (torch.uint8, torch.int8):
+        pool = torch.zeros(4, 16, 2, 64, dtype=bits)
+        assert H.paged_kv(pool, pool, H.F8_E4M3).type == H.F8_E4M3
+    with pytest.raises(ValueError):
+        H.paged_kv(good, good, 12)
+    for order in ("NHD", "HND", "", "hdn", None):
+        with pytest.raises(ValueError):
+            H.paged_kv(good, good, H.F8_E4M3, order=order)
+    for scale in (torch.ones(2, dtype=torch.int32), torch.ones(2, dtype=torch.float64), torch.ones(4, dtype=torch.float16)):
+        with pytest.raises(ValueError):
+            H.paged_kv(good, good, H.F8_E4M3, k_scale=scale)
+        with pytest.raises(ValueError):
+            H.paged_kv(good, good, H.F8_E4M3, v_scale=scale)
