@@ -69,6 +69,7 @@ class PagedKV(C.Structure):
 
 class PagedBatch(C.Structure):
     """c2h_paged_batch: the sessions of a call and their pages."""
+    columns = None  # of a table whose rows lie further apart than that (paged_batch)
     _fields_ = [("block_table", C.c_void_p), ("table_stride", C.c_int64), ("seq_lens", C.c_void_p),
                 ("n_seqs", C.c_int32), ("max_len", C.c_int32)]
 
@@ -410,6 +411,8 @@ class Ctx:
         """Keys and values of new tokens into their pages, K rotated, and the
         queries rotated to q_out (c2h_paged_append_dev)."""
         start = None if token_start is None else _ip(token_start, batch.n_seqs + 1)
+        if batch.columns is not None:
+            _covered(kv, batch)
         rc = _lib.c2h_paged_append_dev(self.h, kv, batch, start, n_tokens, rope, ggml_type, k, v, n_heads, q, q_out)
         if rc:
             self._chk(rc)
@@ -417,6 +420,8 @@ class Ctx:
     def paged_attn_dev(self, kv: PagedKV, batch: PagedBatch, ggml_type: int, n_heads: int, scale: float, q: Heads,
                        out: Heads, window: int = 0):
         """One new token per session over its pages (c2h_paged_attn_dev)."""
+        if batch.columns is not None:
+            _covered(kv, batch)
         rc = _lib.c2h_paged_attn_dev(self.h, kv, batch, ggml_type, n_heads, scale, window, q, out)
         if rc:
             self._chk(rc)
@@ -522,12 +527,23 @@ def paged_batch(block_table, seq_lens, max_len: int) -> PagedBatch:
         raise ValueError("paged_batch() takes a table [sessions, pages] and as many lengths")
     if _KIND[block_table.dtype] != "int32":
         raise ValueError("paged_batch() takes int32 tables")
-    return PagedBatch(block_table.data_ptr(), block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1],
-                      _ip(seq_lens, block_table.shape[0]), seq_lens.shape[0], max_len)
+    rows, columns = block_table.shape
+    b = PagedBatch(block_table.data_ptr(), block_table.stride(0) if rows > 1 else columns, _ip(seq_lens, rows), rows, max_len)
+    if columns < b.table_stride:
+        b.columns = columns
+    return b
+
+
+def _covered(kv, batch):
+    """The library asks that a row's stride cover max_len; here the columns do."""
+    if batch.max_len > batch.columns * kv.page_size:
+        raise ValueError(f"{batch.columns} columns of pages of {kv.page_size} do not cover max_len {batch.max_len}")
 
 
 def paged_attn_workspace(kv: PagedKV, batch: PagedBatch, n_heads: int, window: int = 0) -> int:
     """Bytes of the context's workspace that paged_attn_dev takes."""
+    if batch.columns is not None:
+        _covered(kv, batch)
     n = C.c_size_t()
     rc = lib().c2h_paged_attn_workspace(C.byref(kv), C.byref(batch), n_heads, window, C.byref(n))
     if rc != C2H_OK:

@@ -472,3 +472,30 @@ def test_pools_of_another_element_type_or_order_refused():
             H.paged_kv(good, good, H.F8_E4M3, k_scale=scale)
         with pytest.raises(ValueError):
             H.paged_kv(good, good, H.F8_E4M3, v_scale=scale)
+
+
+def test_tables_of_fewer_columns_than_max_len_takes_refused():
+    """A view of some columns of a wider table covers what its columns cover:
+    pages are not taken from the table's other columns or from behind it."""
+    torch = pytest.importorskip("torch")
+    ctx, x = host_ctx(), heads()
+    wide, lens = torch.ones(3, 8, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    for view in (wide[:, :4], wide[:, 4:], wide[:, 2:6]):
+        good, bad = H.paged_batch(view, lens, 64), H.paged_batch(view, lens, 65)
+        assert (good.table_stride, good.n_seqs) == (8, 3)
+        assert H.paged_attn_workspace(kv(), good, 4) == 0
+        calls = (lambda b: ctx.paged_attn_dev(kv(), b, H.F32, 4, 0.125, x, x),
+                 lambda b: ctx.paged_append_dev(kv(), b, H.F32, 3, x, x))
+        for call in calls:
+            with pytest.raises(H.C2hError, match="no context"):
+                call(good)
+            with pytest.raises(ValueError, match="cover"):
+                call(bad)
+        with pytest.raises(ValueError, match="cover"):
+            H.paged_attn_workspace(kv(), bad, 4)
+    # a single row's stride is its columns; a whole table is the library's to check
+    assert H.paged_batch(wide[:1, :4], lens[:1], 64).table_stride == 4
+    with pytest.raises(H.C2hError, match="cover"):
+        H.paged_attn_workspace(kv(), H.paged_batch(wide[:1, :4], lens[:1], 65), 4)
+    with pytest.raises(H.C2hError, match="cover"):
+        H.paged_attn_workspace(kv(), H.paged_batch(wide, lens, 129), 4)
