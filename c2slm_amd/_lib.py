@@ -44,6 +44,8 @@ class ModelDesc(C.Structure):
 
 class Heads(C.Structure):
     """c2h_heads: head vectors of a run of tokens in device memory."""
+    of = None    # element type, tokens, heads and head_dim of the tensor that heads() took
+    fits = None  # the call's type, tokens, heads and head_dim that they were last found to cover
     _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
@@ -400,6 +402,11 @@ class Ctx:
     def rope_dev(self, rope: Rope, ggml_type: int, x: Heads, positions, n_tokens: int, n_heads: int, head_dim: int,
                  y: Heads):
         """y = x rotated to positions (c2h_rope_dev)."""
+        want = (ggml_type, n_tokens, n_heads, head_dim)
+        if x is not None and x.fits != want:
+            _hold(x, want)
+        if y is not None and y.fits != want:
+            _hold(y, want)
         at = None if positions is None else _ip(positions, n_tokens)
         rc = _lib.c2h_rope_dev(self.h, rope, ggml_type, x, at, n_tokens, n_heads, head_dim, y)
         if rc:
@@ -410,6 +417,17 @@ class Ctx:
                          n_heads: int = 0):
         """Keys and values of new tokens into their pages, K rotated, and the
         queries rotated to q_out (c2h_paged_append_dev)."""
+        dim = kv.head_dim
+        want = (ggml_type, n_tokens, kv.n_kv_heads, dim)
+        if k is not None and k.fits != want:
+            _hold(k, want)
+        if v is not None and v.fits != want:
+            _hold(v, want)
+        want = (ggml_type, n_tokens, n_heads, dim)
+        if q is not None and q.fits != want:
+            _hold(q, want)
+        if q_out is not None and q_out.fits != want:
+            _hold(q_out, want)
         start = None if token_start is None else _ip(token_start, batch.n_seqs + 1)
         if batch.columns is not None:
             _covered(kv, batch)
@@ -420,6 +438,11 @@ class Ctx:
     def paged_attn_dev(self, kv: PagedKV, batch: PagedBatch, ggml_type: int, n_heads: int, scale: float, q: Heads,
                        out: Heads, window: int = 0):
         """One new token per session over its pages (c2h_paged_attn_dev)."""
+        want = (ggml_type, batch.n_seqs, n_heads, kv.head_dim)
+        if q is not None and q.fits != want:
+            _hold(q, want)
+        if out is not None and out.fits != want:
+            _hold(out, want)
         if batch.columns is not None:
             _covered(kv, batch)
         rc = _lib.c2h_paged_attn_dev(self.h, kv, batch, ggml_type, n_heads, scale, window, q, out)
@@ -483,7 +506,20 @@ def heads(t) -> Heads:
     are; elements of a head contiguous)."""
     if t.ndim != 3 or t.stride(2) != 1:
         raise ValueError("heads() takes [tokens, heads, head_dim] with contiguous elements")
-    return Heads(t.data_ptr(), t.stride(0), t.stride(1))
+    h = Heads(t.data_ptr(), t.stride(0), t.stride(1))
+    h.of = (_KIND[t.dtype], *t.shape)
+    return h
+
+
+def _hold(h, want):
+    """Whether the vectors a call takes lie within the tensor that heads()
+    took; asked again only where a call's description differs."""
+    if h.of is not None:
+        (ggml_type, n_tokens, n_heads, head_dim), (element, tokens, n, dim) = want, h.of
+        if element != ELEMENT.get(ggml_type) or tokens < n_tokens or n < n_heads or dim < head_dim:
+            raise ValueError(f"{n_tokens} tokens of {n_heads} heads of {head_dim} elements of type {ggml_type} in a tensor "
+                             f"{[tokens, n, dim]} of {element}")
+    h.fits = want
 
 
 def rope(rot_dim: int, base: float, layout: str = "half", factor: float = 1.0, orig_ctx: int = 0,

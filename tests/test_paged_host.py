@@ -499,3 +499,42 @@ def test_tables_of_fewer_columns_than_max_len_takes_refused():
         H.paged_attn_workspace(kv(), H.paged_batch(wide[:1, :4], lens[:1], 65), 4)
     with pytest.raises(H.C2hError, match="cover"):
         H.paged_attn_workspace(kv(), H.paged_batch(wide, lens, 129), 4)
+
+
+def test_calls_beyond_the_tensor_that_heads_took_refused():
+    """The type, tokens, heads and width that a call names have to lie within
+    the tensor; what heads() did not make is taken as it is described."""
+    torch = pytest.importorskip("torch")
+    ctx, rope, at = host_ctx(), H.rope(64, 1e6), torch.zeros(3, dtype=torch.int32)
+    t = lambda *shape, dtype=torch.float32: H.heads(torch.zeros(*shape, dtype=dtype))  # noqa: E731
+    small = [t(2, 4, 64), t(3, 1, 64), t(3, 4, 48), t(3, 4, 64, dtype=torch.bfloat16), t(3, 4, 64, dtype=torch.float16),
+             t(3, 4, 64, dtype=torch.int32), t(3, 4, 64, dtype=torch.float64)]
+    kv2 = kv()
+
+    def calls(h):
+        """Each place of each call with h there, the rest fitting."""
+        x = lambda: t(3, 4, 64)  # noqa: E731
+        return [lambda: ctx.rope_dev(rope, H.F32, h, at, 3, 4, 64, x()), lambda: ctx.rope_dev(rope, H.F32, x(), at, 3, 4, 64, h),
+                lambda: ctx.paged_append_dev(kv2, batch(), H.F32, 3, h, x()),
+                lambda: ctx.paged_append_dev(kv2, batch(), H.F32, 3, x(), h),
+                lambda: ctx.paged_append_dev(kv2, batch(), H.F32, 3, x(), x(), q=h, q_out=x(), n_heads=4),
+                lambda: ctx.paged_append_dev(kv2, batch(), H.F32, 3, x(), x(), q=x(), q_out=h, n_heads=4),
+                lambda: ctx.paged_attn_dev(kv2, batch(), H.F32, 4, 0.125, h, x()),
+                lambda: ctx.paged_attn_dev(kv2, batch(), H.F32, 4, 0.125, x(), h)]
+
+    for bad in small:
+        for call in calls(bad):
+            with pytest.raises(ValueError):
+                call()
+    for good in (t(3, 4, 64), t(5, 6, 80), heads()):
+        for call in calls(good):
+            with pytest.raises(H.C2hError, match="no context"):
+                call()
+    # found to fit one call does not answer for another
+    good = t(3, 4, 64)
+    for _ in range(2):
+        for n, n_heads, dim, ty in ((3, 4, 64, H.F32), (4, 4, 64, H.F32), (3, 5, 64, H.F32), (3, 4, 72, H.F32),
+                                    (3, 4, 64, H.BF16), (3, 4, 64, H.F16)):
+            fits = (n, n_heads, dim, ty) == (3, 4, 64, H.F32)
+            with pytest.raises(H.C2hError if fits else ValueError):
+                ctx.rope_dev(rope, ty, good, torch.zeros(9, dtype=torch.int32), n, n_heads, dim, heads())
