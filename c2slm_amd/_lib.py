@@ -44,8 +44,8 @@ class ModelDesc(C.Structure):
 
 class Heads(C.Structure):
     """c2h_heads: head vectors of a run of tokens in device memory."""
-    of = None    # element type, tokens, heads and head_dim of the tensor that heads() took
-    fits = None  # the call's type, tokens, heads and head_dim that they were last found to cover
+    of = None    # element type, tokens, heads, head_dim and GPU of the tensor that heads() took
+    fits = None  # the call's type, tokens, heads, head_dim and GPU that they were last found to cover
     _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
@@ -63,6 +63,7 @@ class Rope(C.Structure):
 
 class PagedKV(C.Structure):
     """c2h_paged_kv: a pool of pages of keys and values."""
+    device = None  # the GPU of the tensors that paged_kv() took
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + \
                [(n, C.c_int32) for n in ("type", "n_pages", "page_size", "n_kv_heads", "head_dim", "reserved")] + \
                [(n, C.c_int64) for n in ("page_stride", "token_stride", "head_stride")] + \
@@ -72,6 +73,7 @@ class PagedKV(C.Structure):
 class PagedBatch(C.Structure):
     """c2h_paged_batch: the sessions of a call and their pages."""
     columns = None  # of a table whose rows lie further apart than that (paged_batch)
+    device = None   # the GPU of the tensors that paged_batch() took
     _fields_ = [("block_table", C.c_void_p), ("table_stride", C.c_int64), ("seq_lens", C.c_void_p),
                 ("n_seqs", C.c_int32), ("max_len", C.c_int32)]
 
@@ -164,6 +166,7 @@ def _p(a: np.ndarray):
 
 class Ctx:
     """One c2h context (one device stream, its buffers)."""
+    device = 0
 
     def __init__(self, desc: ModelDesc | None = None, device: int = 0):
         L = lib()
@@ -173,6 +176,7 @@ class Ctx:
             raise C2hError(rc, (L.c2h_last_error(None) or b"").decode())
         self.h = h
         self.desc = desc
+        self.device = device
 
     def _chk(self, rc: int):
         if rc != C2H_OK:
@@ -402,12 +406,12 @@ class Ctx:
     def rope_dev(self, rope: Rope, ggml_type: int, x: Heads, positions, n_tokens: int, n_heads: int, head_dim: int,
                  y: Heads):
         """y = x rotated to positions (c2h_rope_dev)."""
-        want = (ggml_type, n_tokens, n_heads, head_dim)
+        want = (ggml_type, n_tokens, n_heads, head_dim, self.device)
         if x is not None and x.fits != want:
             _hold(x, want)
         if y is not None and y.fits != want:
             _hold(y, want)
-        at = None if positions is None else _ip(positions, n_tokens)
+        at = None if positions is None else _ip(positions, n_tokens, self.device)
         rc = _lib.c2h_rope_dev(self.h, rope, ggml_type, x, at, n_tokens, n_heads, head_dim, y)
         if rc:
             self._chk(rc)
@@ -417,18 +421,20 @@ class Ctx:
                          n_heads: int = 0):
         """Keys and values of new tokens into their pages, K rotated, and the
         queries rotated to q_out (c2h_paged_append_dev)."""
-        dim = kv.head_dim
-        want = (ggml_type, n_tokens, kv.n_kv_heads, dim)
+        dim, device = kv.head_dim, self.device
+        if kv.device != device or batch.device != device:
+            _here(device, kv, batch)
+        want = (ggml_type, n_tokens, kv.n_kv_heads, dim, device)
         if k is not None and k.fits != want:
             _hold(k, want)
         if v is not None and v.fits != want:
             _hold(v, want)
-        want = (ggml_type, n_tokens, n_heads, dim)
+        want = (ggml_type, n_tokens, n_heads, dim, device)
         if q is not None and q.fits != want:
             _hold(q, want)
         if q_out is not None and q_out.fits != want:
             _hold(q_out, want)
-        start = None if token_start is None else _ip(token_start, batch.n_seqs + 1)
+        start = None if token_start is None else _ip(token_start, batch.n_seqs + 1, device)
         if batch.columns is not None:
             _covered(kv, batch)
         rc = _lib.c2h_paged_append_dev(self.h, kv, batch, start, n_tokens, rope, ggml_type, k, v, n_heads, q, q_out)
@@ -438,7 +444,10 @@ class Ctx:
     def paged_attn_dev(self, kv: PagedKV, batch: PagedBatch, ggml_type: int, n_heads: int, scale: float, q: Heads,
                        out: Heads, window: int = 0):
         """One new token per session over its pages (c2h_paged_attn_dev)."""
-        want = (ggml_type, batch.n_seqs, n_heads, kv.head_dim)
+        device = self.device
+        if kv.device != device or batch.device != device:
+            _here(device, kv, batch)
+        want = (ggml_type, batch.n_seqs, n_heads, kv.head_dim, device)
         if q is not None and q.fits != want:
             _hold(q, want)
         if out is not None and out.fits != want:
@@ -454,16 +463,18 @@ class Ctx:
         rows and, where y is given, floats (c2h_rmsnorm_q8k_dev)."""
         n, cols = x.shape
         xs, one = x.stride()
-        own = x.dtype
+        own, device = x.dtype, self.device
         if one != 1 or _KIND[own] != ELEMENT.get(ggml_type):
             raise ValueError("rmsnorm_q8k_dev() takes rows of the call's type, their elements contiguous")
         if _KIND[w.dtype] != "float32" or (y is not None and _KIND[y.dtype] != "float32"):
             raise ValueError("rmsnorm_q8k_dev() takes w and y of float32")
-        rp, rs = _rows(residual, n, cols, own) if residual is not None else (None, 0)
-        sp, ss = _rows(sum_out, n, cols, own) if sum_out is not None else (None, 0)
-        yp, ys = _rows(y, n, cols, y.dtype) if y is not None else (None, 0)
+        rp, rs = _rows(residual, n, cols, own, device) if residual is not None else (None, 0)
+        sp, ss = _rows(sum_out, n, cols, own, device) if sum_out is not None else (None, 0)
+        yp, ys = _rows(y, n, cols, y.dtype, device) if y is not None else (None, 0)
         if w.numel() != cols or not w.is_contiguous() or q8k.nbytes < n * (cols // 256) * 292 or not q8k.is_contiguous():
             raise ValueError("rmsnorm_q8k_dev() takes a weight per column and 292 bytes per 256 of them in each row")
+        if x.get_device() != device or w.get_device() != device or q8k.get_device() != device:
+            raise ValueError(ELSEWHERE)
         rc = _lib.c2h_rmsnorm_q8k_dev(self.h, ggml_type, x.data_ptr(), xs, rp, rs, w.data_ptr(), eps, n, cols, sp, ss,
                                       q8k.data_ptr(), yp, ys)
         if rc:
@@ -479,25 +490,36 @@ class _Kinds(dict):
 
 
 _KIND = _Kinds()
+ELSEWHERE = "the operators over many sessions take tensors on the context's GPU"
+
+
+def _here(device, *described):
+    for d in described:
+        if d.device is not None and d.device != device:
+            raise ValueError(ELSEWHERE)
 
 
 def _dp(t):
     return None if t is None else t.data_ptr()
 
 
-def _ip(t, n):
+def _ip(t, n, device):
     """Address of n positions or the like: int32, one after another."""
     if _KIND[t.dtype] != "int32" or t.numel() < n or not t.is_contiguous():
         raise ValueError("positions, lengths and starts are contiguous int32: one per token or session, starts one more")
+    if t.get_device() != device:
+        raise ValueError(ELSEWHERE)
     return t.data_ptr()
 
 
-def _rows(t, n, cols, dtype):
+def _rows(t, n, cols, dtype, device):
     """Address and stride of the (first) n rows of a tensor of cols columns."""
     stride, one = t.stride()
     rows, width = t.shape
     if one != 1 or rows < n or width != cols or t.dtype is not dtype:
         raise ValueError("rows and columns as x has them, of its type, their elements contiguous")
+    if t.get_device() != device:
+        raise ValueError(ELSEWHERE)
     return t.data_ptr(), stride
 
 
@@ -507,7 +529,7 @@ def heads(t) -> Heads:
     if t.ndim != 3 or t.stride(2) != 1:
         raise ValueError("heads() takes [tokens, heads, head_dim] with contiguous elements")
     h = Heads(t.data_ptr(), t.stride(0), t.stride(1))
-    h.of = (_KIND[t.dtype], *t.shape)
+    h.of = (_KIND[t.dtype], *t.shape, t.get_device())
     return h
 
 
@@ -515,7 +537,9 @@ def _hold(h, want):
     """Whether the vectors a call takes lie within the tensor that heads()
     took; asked again only where a call's description differs."""
     if h.of is not None:
-        (ggml_type, n_tokens, n_heads, head_dim), (element, tokens, n, dim) = want, h.of
+        (ggml_type, n_tokens, n_heads, head_dim, device), (element, tokens, n, dim, place) = want, h.of
+        if place != device:
+            raise ValueError(ELSEWHERE)
         if element != ELEMENT.get(ggml_type) or tokens < n_tokens or n < n_heads or dim < head_dim:
             raise ValueError(f"{n_tokens} tokens of {n_heads} heads of {head_dim} elements of type {ggml_type} in a tensor "
                              f"{[tokens, n, dim]} of {element}")
@@ -552,8 +576,13 @@ def paged_kv(k, v, ggml_type: int, order: str = "nhd", k_scale=None, v_scale=Non
     for scale in (k_scale, v_scale):
         if scale is not None and (_KIND[scale.dtype] != "float32" or not scale.is_contiguous() or scale.numel() != k.shape[h]):
             raise ValueError("paged_kv() takes a float32 scale per KV head")
-    return PagedKV(k.data_ptr(), v.data_ptr(), ggml_type, k.shape[0], k.shape[t], k.shape[h], k.shape[3], 0, k.stride(0),
-                   k.stride(t), k.stride(h), _dp(k_scale), _dp(v_scale))
+    devices = {x.get_device() for x in (k, v, k_scale, v_scale) if hasattr(x, "get_device")}
+    if len(devices) > 1:
+        raise ValueError("paged_kv() takes pools and scales on one GPU")
+    kv = PagedKV(k.data_ptr(), v.data_ptr(), ggml_type, k.shape[0], k.shape[t], k.shape[h], k.shape[3], 0, k.stride(0),
+                 k.stride(t), k.stride(h), _dp(k_scale), _dp(v_scale))
+    kv.device = devices.pop() if devices else None
+    return kv
 
 
 def paged_batch(block_table, seq_lens, max_len: int) -> PagedBatch:
@@ -564,7 +593,10 @@ def paged_batch(block_table, seq_lens, max_len: int) -> PagedBatch:
     if _KIND[block_table.dtype] != "int32":
         raise ValueError("paged_batch() takes int32 tables")
     rows, columns = block_table.shape
-    b = PagedBatch(block_table.data_ptr(), block_table.stride(0) if rows > 1 else columns, _ip(seq_lens, rows), rows, max_len)
+    device = block_table.get_device()
+    b = PagedBatch(block_table.data_ptr(), block_table.stride(0) if rows > 1 else columns, _ip(seq_lens, rows, device), rows,
+                   max_len)
+    b.device = device
     if columns < b.table_stride:
         b.columns = columns
     return b

@@ -392,9 +392,10 @@ def test_python_tensors_of_other_shapes_and_types_refused():
 
 
 def host_ctx():
-    """A context that no call reaches: every call here is refused before."""
+    """A context that no call reaches: every call here is refused before.  The
+    tensors' device, the CPU's -1, stands for the context's GPU."""
     ctx = object.__new__(H.Ctx)
-    ctx.h = None
+    ctx.h, ctx.device = None, -1
     return ctx
 
 
@@ -538,3 +539,56 @@ def test_calls_beyond_the_tensor_that_heads_took_refused():
             fits = (n, n_heads, dim, ty) == (3, 4, 64, H.F32)
             with pytest.raises(H.C2hError if fits else ValueError):
                 ctx.rope_dev(rope, ty, good, torch.zeros(9, dtype=torch.int32), n, n_heads, dim, heads())
+
+
+def test_tensors_that_are_not_on_the_contexts_gpu_refused():
+    """A CPU tensor, or one of another GPU, would fault in the kernel."""
+    torch = pytest.importorskip("torch")
+    ctx, rope = host_ctx(), H.rope(64, 1e6)
+    f, i = (lambda *s: torch.zeros(*s)), (lambda *s: torch.zeros(*s, dtype=torch.int32))
+    pool = torch.zeros(4, 16, 2, 64, dtype=torch.uint8)
+    norm = dict(x=f(3, 512), w=f(512), q8k=torch.zeros(3, 2, 292, dtype=torch.uint8), residual=f(3, 512), sum_out=f(3, 512), y=f(3, 512))
+
+    class Elsewhere:
+        """t, on GPU 1."""
+
+        def __init__(self, t):
+            self.t = t
+
+        def get_device(self):
+            return 1
+
+        def __getattr__(self, name):
+            return getattr(self.t, name)
+
+    def calls(x=heads(), y=heads(), pos=i(3), start=i(4), kv_=kv(), batch_=batch(), **more):
+        return [lambda: ctx.rope_dev(rope, H.F32, x, pos, 3, 4, 64, y),
+                lambda: ctx.paged_append_dev(kv_, batch_, H.F32, 3, x, y, token_start=start, q=y, q_out=x, n_heads=4),
+                lambda: ctx.paged_attn_dev(kv_, batch_, H.F32, 4, 0.125, x, y),
+                lambda: ctx.rmsnorm_q8k_dev(H.F32, eps=1e-6, **dict(norm, **more))]
+
+    def said(call):
+        with pytest.raises((ValueError, H.C2hError)) as e:
+            call()
+        return "GPU" if "GPU" in str(e.value) else "context" if "no context" in str(e.value) else str(e.value)
+
+    own = dict(x=H.heads(f(3, 4, 64)), kv_=H.paged_kv(pool, pool.clone(), H.F8_E4M3, k_scale=f(2)), batch_=H.paged_batch(i(3, 8), i(3), 128))
+    assert [said(c) for c in calls(**{**own, "x": heads()})] == ["context"] * 4
+    assert said(calls(x=own["x"])[0]) == "context"
+    far = dict(x=H.heads(Elsewhere(f(3, 4, 64))), y=H.heads(Elsewhere(f(3, 4, 64))),
+               kv_=H.paged_kv(Elsewhere(pool), Elsewhere(pool.clone()), H.F8_E4M3), batch_=H.paged_batch(Elsewhere(i(3, 8)), Elsewhere(i(3)), 128))
+    for name, which in (("x", (0, 1, 2)), ("y", (0, 1, 2)), ("kv_", (1, 2)), ("batch_", (1, 2))):
+        got = [said(c) for c in calls(**{name: far[name]})[:3]]
+        assert got == ["GPU" if n in which else "context" for n in range(3)], (name, got)
+    assert said(calls(pos=Elsewhere(i(3)))[0]) == "GPU" and said(calls(start=Elsewhere(i(4)))[1]) == "GPU"
+    for name in norm:
+        x = norm[name]
+        assert said(lambda: ctx.rmsnorm_q8k_dev(H.F32, eps=1e-6, **dict(norm, **{name: Elsewhere(x)}))) == "GPU", name
+    for bad in (dict(k=Elsewhere(pool), v=pool), dict(k=pool, v=pool, k_scale=Elsewhere(f(2))), dict(k=pool, v=pool, v_scale=Elsewhere(f(2)))):
+        with pytest.raises(ValueError, match="GPU"):
+            H.paged_kv(ggml_type=H.F8_E4M3, **bad)
+    with pytest.raises(ValueError, match="GPU"):
+        H.paged_batch(i(3, 8), Elsewhere(i(3)), 128)
+    # a context of a GPU takes nothing of the CPU's
+    ctx.device = 0
+    assert [said(c) for c in calls(**own)] == ["GPU"] * 4
