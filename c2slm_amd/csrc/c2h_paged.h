@@ -59,10 +59,12 @@ C2H_HD constexpr int attn_tiles(int type, int hd) {
 C2H_HD constexpr int attn_hd(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 C2H_HD constexpr int attn_unit(int type, int head_dim) { return 64 * attn_tiles(type, attn_hd(head_dim)); }
 // Units per chunk: a batch of `units` in all, in each of n_rows (KV head, head
-// tile) rows, as about ATTN_CHUNKS equal chunks.
+// tile) rows, as about ATTN_CHUNKS equal chunks; no more than the longest
+// session has of the smallest unit, so that a chunk's positions (at most 2^25)
+// fit 32 bits however large the batch.
 C2H_HD inline int chunk_units(int64_t units, int n_rows) {
-  const int64_t c = (units * n_rows + ATTN_CHUNKS - 1) / ATTN_CHUNKS;
-  return (int)(c < 1 ? 1 : c);
+  const int64_t c = (units * n_rows + ATTN_CHUNKS - 1) / ATTN_CHUNKS, most = PAGED_MAX_LEN / 64;
+  return (int)(c < 1 ? 1 : c < most ? c : most);
 }
 // Chunks (of one row) that any batch of sessions of up to max_units can come
 // to: about ATTN_CHUNKS / n_rows, and a partial one per session.

@@ -592,3 +592,44 @@ def test_tensors_that_are_not_on_the_contexts_gpu_refused():
     # a context of a GPU takes nothing of the CPU's
     ctx.device = 0
     assert [said(c) for c in calls(**own)] == ["GPU"] * 4
+
+
+LARGEST = r"""
+#include <initializer_list>
+#include <cassert>
+#include <cstdio>
+#include "c2h_paged.h"
+using namespace c2h;
+int main() {
+  // batches up to the largest that a call accepts: a chunk's positions, and
+  // the positions that a session's chunks begin and end at, fit 32 bits, and
+  // the chunks cover the session
+  for (int unit : {64, 128, 256})
+    for (int n_seqs : {1, 64, 1000, 16383, 65535})
+      for (int n_rows : {1, 16, 256, 1024, 4096})
+        for (int len : {1, 5000, 131072, 140000, 1 << 20, PAGED_MAX_LEN - 1, PAGED_MAX_LEN}) {
+          if ((int64_t)n_seqs * n_rows > MAX_SESSION_HEADS) continue;
+          const Span s = attended(len, 0);
+          const int units = units_of(s, unit), cu = chunk_units((int64_t)units * n_seqs, n_rows);
+          const int chunk = cu * unit, n = chunks_of(units, cu);  // as the kernel computes it
+          assert(cu >= 1 && chunk >= unit && n >= 1 && (int64_t)n * n_seqs <= chunks_bound(n_seqs, n_rows, units));
+          int at = 0;
+          for (int i = 0; i < n; ++i) {
+            const int b = chunk_base(s, chunk, i), e = b + chunk < s.hi ? b + chunk : s.hi;
+            assert(b == at && e > b);
+            at = e;
+          }
+          assert(at == len);
+        }
+  puts("ok");
+}
+"""
+
+
+def test_chunks_of_the_largest_batches(tmp_path):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(LARGEST)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover=all", "-I",
+                    os.path.join(ROOT, "c2slm_amd", "csrc"), str(src), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert run.returncode == 0 and run.stdout == "ok\n", run.stderr
