@@ -2624,7 +2624,9 @@ int check_paged(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b) {
     return fail(c, C2H_ERR_INVALID, "cache vectors overlap");
   if (b->n_seqs < 0 || b->n_seqs > 65535) return fail(c, C2H_ERR_INVALID, "%d sessions: up to 65535", b->n_seqs);
   if (b->max_len < 0 || b->max_len > PAGED_MAX_LEN) return fail(c, C2H_ERR_INVALID, "max_len %d", b->max_len);
-  if (b->n_seqs > 0 && (!b->block_table || !b->seq_lens)) return fail(c, C2H_ERR_INVALID, "no block table or lengths");
+  // a table of no columns, where every session is empty, may have no memory
+  if (b->n_seqs > 0 && ((!b->block_table && b->max_len > 0) || !b->seq_lens))
+    return fail(c, C2H_ERR_INVALID, "no block table or lengths");
   if (!stride_fits(b->table_stride, b->n_seqs, 4) ||
       b->table_stride < ((int64_t)b->max_len + kv->page_size - 1) / kv->page_size)
     return fail(c, C2H_ERR_INVALID, "a table row of %lld pages of %d tokens does not cover max_len %d",

@@ -363,7 +363,8 @@ typedef struct c2h_paged_kv {
  * seq_lens[s] positions, the call's own new ones included (0: no session in
  * this row).  Table and lengths are device int32 and may change between
  * calls; max_len, up to 2^23, is a bound of the lengths that the host knows
- * (the launch is sized by it; table_stride * page_size covers it).
+ * (the launch is sized by it; table_stride * page_size covers it; where it is
+ * 0, no session holds a position and block_table may be NULL).
  * The kernels check what they find there: a length below 0 or above
  * max_len, or a page index outside [0, n_pages) where a position is held,
  * reads and writes nothing outside the pool; such a session's attention

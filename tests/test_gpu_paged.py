@@ -811,3 +811,29 @@ def test_attention_block_of_a_layer(ctx, cache):
         assert ((att.cpu().double() - want).abs() <= tol).all()
         for s in range(3):
             assert np.array_equal(aq[s].cpu().numpy().ravel(), O.quantize_row_q8k(att[s].cpu().numpy().ravel()))
+
+
+def test_batch_of_empty_sessions_without_pages(ctx):
+    # no session holds a position: a table of no columns, rows of zeros,
+    # queries left as they were; a length that is not 0 is reported
+    sess = Sessions([4], 2, 64, 16, "nhd", H.BF16, 1)
+    kv, _ = sess.cuda()
+    before = [d.clone() for d in sess.dev]
+    table = torch.zeros((3, 0), dtype=torch.int32, device="cuda")
+    x = torch.randn(3, 4, 64, device="cuda")
+    for lens, bad in (([0, 0, 0], []), ([0, 5, -1], [1, 2])):
+        lens_d = torch.tensor(lens, dtype=torch.int32).cuda()
+        out, qo = torch.full_like(x, 5.0), torch.full_like(x, 5.0)
+        batch = H.paged_batch(table, lens_d, 0)
+        torch.cuda.synchronize()
+        ctx.paged_append_dev(kv, batch, H.F32, 3, H.heads(x[:, :2]), H.heads(x[:, 2:]), q=H.heads(x), q_out=H.heads(qo), n_heads=4)
+        ctx.paged_attn_dev(kv, batch, H.F32, 4, 0.125, H.heads(x), H.heads(out))
+        if bad:
+            with pytest.raises(H.C2hError, match="length"):
+                ctx.sync()
+        else:
+            ctx.sync()
+        assert (qo == 5.0).all()
+        for s in range(3):
+            assert torch.isnan(out[s]).all() if s in bad else (out[s] == 0.0).all()
+    assert all(torch.equal(Sessions.bits(d), Sessions.bits(b)) for d, b in zip(sess.dev, before))

@@ -633,3 +633,14 @@ def test_chunks_of_the_largest_batches(tmp_path):
                     os.path.join(ROOT, "c2slm_amd", "csrc"), str(src), "-o", str(exe)], check=True)
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and run.stdout == "ok\n", run.stderr
+
+
+def test_batch_of_empty_sessions_without_pages():
+    """max_len 0: no session holds a position, and the table may be empty."""
+    L, n, q = H.lib(), C.c_size_t(7), heads()
+    none = batch(block_table=None, table_stride=0, max_len=0)
+    assert L.c2h_paged_attn_workspace(kv(), none, 4, 0, C.byref(n)) == 0 and n.value == 0
+    refused(L.c2h_paged_attn_dev(None, kv(), none, H.F32, 4, 0.125, 0, q, q), INVALID, "no context")
+    refused(L.c2h_paged_append_dev(None, kv(), none, None, 3, None, H.F32, q, q, 0, None, None), INVALID, "no context")
+    refused(L.c2h_paged_attn_dev(None, kv(), batch(block_table=None, table_stride=0, max_len=0, seq_lens=None), H.F32, 4, 0.125, 0,
+                                 q, q), INVALID, "lengths")
