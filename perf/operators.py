@@ -13,6 +13,12 @@ generic ones, from one session's step to batches of long sessions.
 run() computes the operators in elementary torch operations in 32 bits
 (angles and squared sums in 64) where `own` is false, and calls the package
 where it is true.  exact() is each operator's definition in 64 bits.
+
+The package's calls run on the context's stream, which torch's streams do not
+wait for.  prepare() returns once the inputs are complete, and run() queues its
+call as a layer of a decode step does, without a wait: who uses its outputs
+waits first, for the device (torch.cuda.synchronize()) or for the context
+(sync(), which also reports a page or length out of range).
 """
 import math
 import random
@@ -248,6 +254,13 @@ def _code(H, ty):
 
 
 def prepare(case, seed):
+    st = _prepared(case, seed)
+    if own:
+        torch.cuda.synchronize()  # the context's stream reads what torch's wrote
+    return st
+
+
+def _prepared(case, seed):
     kind = case["kind"]
     if kind == "rope":
         g, n = _gen(seed), case["tokens"]
