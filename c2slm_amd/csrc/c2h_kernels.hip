@@ -573,8 +573,8 @@ __device__ __forceinline__ float4 store_row4(char* row, int i, int cols, float4 
 // takes them; the row is read once and stays in registers.  The squares are
 // summed in 64 bits, so that the order of the sum does not reach the quants.
 // Bound by memory: 8,192 rows of 2,048 bf16 with residual, quants and f32 rows
-// (187 MB) 39.8 us, 4.7 TB/s, what a large copy reaches; one row of 896 is 2.3
-// us, launch and one chain of loads.  Tried: streamed loads 38.3 (but x is
+// (187 MB) 40.4 us, 4.6 TB/s, near what a large copy reaches (4.7); one row of
+// 896 is 2.2 us, launch and one chain of loads.  Tried: streamed loads 38.3 (but x is
 // fresh in the caches where a layer runs), the weights loaded before the sum
 // 40.3.
 template <int T, int BPW, int NW, bool VEC>

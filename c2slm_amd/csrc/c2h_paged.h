@@ -23,7 +23,7 @@ constexpr int PAGED_MAX_PAGE = 1024;
 // A launch's work-items stay below 2^32, at most 256 per token, per (session,
 // head) and 1024 per row.
 constexpr int MAX_TOKENS = (1 << 24) - 1, MAX_SESSION_HEADS = (1 << 24) - 1, MAX_NORM_ROWS = (1 << 22) - 1;
-constexpr int PAGED_MAX_LEN = 1 << 23; // chunks are a grid's third index
+constexpr int PAGED_MAX_LEN = 1 << 23; // a position and a chunk's end beyond it (chunk_units) fit 32 bits
 constexpr int ATTN_HEADS = 16;         // query heads of a workgroup: columns of the matrix instruction
 constexpr int ATTN_CHUNKS = 1024;      // chunks that a batch is cut into
 constexpr int ATTN_MANY_ROWS = 2048;   // rows from which the join takes several a workgroup

@@ -500,14 +500,21 @@ __device__ __forceinline__ Cut cut_batch(const int32_t* lens, int n_seqs, int ma
 // go round its four waves, and a row of one chunk is written here, others'
 // parts are joined by k_paged_join.
 // Bound by memory where there is much to read: 8 sessions of 32,768 positions,
-// 16/8 heads of 128, f16 in pages of 64 (1,059 MB) 163 us, 6.5 TB/s; 64
-// sessions of 30 to 8,000, 12/2 heads, bf16 (92 MB) 18.7 us, 4.9 TB/s; 128 of
-// up to 4,096, 16/2 heads, e4m3 (161 MB) 39.8 us, 4.1 TB/s.  The matrix units
-// are busy 8 % of that, the VALU 20 to 37 %.  Otherwise by the chain length ->
-// page -> keys: one session of 41 5.0 us, of 4,096 7.8 us.  16 KB a wave and
-// two workgroups to a CU keep 32 MB in flight, more than the memory's latency
-// times its rate; 512 workgroups and 1,024 chunks took 21.2 us where 512
-// chunks took 25.1 and 2,048 24.6 (64 sessions, with the join).
+// 16/8 heads of 128, f16 in pages of 64 (1,059 MB) 163 us, 6.5 TB/s, what a
+// plain streaming read of 4 GiB reaches.  Smaller calls lose to the chain
+// length -> page -> keys at the start of a workgroup's chunks, of a few steps
+// each: 64 sessions of 30 to 8,000, 12/2 heads, bf16 (92 MB) 18.7 us, 4.9 TB/s
+// (a plain read of 100 MB: 5.6); 128 of up to 4,096, 16/2 heads, e4m3 (161 MB)
+// 39.8 us, 4.1 TB/s.  One session of 41 positions, 5.0 us, and one of 4,096,
+// 7.8 us, are that chain.  The matrix units are busy 8 %, the VALU 20 to 37 %.
+// 16 KB a wave and two workgroups to a CU keep 32 MB in flight, more than the
+// memory's latency times its rate; 512 workgroups and 1,024 chunks took 21.2
+// us where 512 chunks took 25.1 and 2,048 24.6 (64 sessions, with the join).
+// More than 16 query heads to a KV head are tiles of 16, a workgroup each that
+// reads the keys and values again: 400 MB in 145 us at 24/1 heads of 128 for
+// 83 at 16/1, and in 143 (plain loads) and 167 us (streamed ones, which the
+// second tile does not find in the cache) at 40/2 heads of 64 for 85 and 80 at
+// 14/2.
 //
 // The leading arguments arrive in registers at wave start (kernel-argument
 // preload).  shape: log2 of the page size; from bit 4: whether sessions can
@@ -1043,7 +1050,12 @@ void launch_attn_as(const PagedAttnParams& P, hipStream_t st) {
 
 // Queries and outputs that a single 16-bit part holds take the shorter
 // split: the pool's own type, and either 16-bit type on f16 and e4m3 pools
-// (a bf16 query fits f16's bits once its range is brought in).
+// (a bf16 query fits f16's bits once its range is brought in).  Widths that
+// fill no template take the longer split and plain loads whatever the types,
+// one kernel a pool type and template: the second product is hidden behind the
+// loads there too (400 MB of bf16, heads' tokens back to back: 10/5 heads of 80
+// 84 us with bf16 rows and with f32, 6/2 of 96 79, 8/4 of 192 94; full widths
+// of 128 and 256 83 and 75).
 template <int CT, int HD>
 void launch_attn_hd(const PagedAttnParams& P, hipStream_t st) {
   if (P.kv.head_dim != HD) return launch_attn_as<CT, HD, false, true, false>(P, st);

@@ -327,9 +327,9 @@ int c2h_rope_init(const c2h_rope_desc* desc, c2h_rope* rope);
 
 /* y = x rotated, for n_tokens tokens of n_heads heads of head_dim elements
  * (a multiple of 8 up to 256, at least rot_dim) of type F32, F16 or BF16;
- * token t stands at positions[t] (device, int32); up to 2^24 - 1 tokens.  32-bit arithmetic, one
- * rounding to the type.  y may be x itself (same pointer and strides);
- * otherwise they must not overlap. */
+ * token t stands at positions[t] (device, int32).  Up to 2^24 - 1 tokens a
+ * call.  32-bit arithmetic, one rounding to the type.  y may be x itself
+ * (same pointer and strides); otherwise they must not overlap. */
 int c2h_rope_dev(c2h_ctx* ctx, const c2h_rope* rope, int32_t type, const c2h_heads* x, const int32_t* positions,
                  int32_t n_tokens, int32_t n_heads, int32_t head_dim, const c2h_heads* y);
 
@@ -388,8 +388,9 @@ typedef struct c2h_paged_batch {
  * none), n_heads vectors per token, goes to q_out, rotated, in `type`;
  * q_out may be q (same pointer and strides).  Tokens from
  * token_start[n_seqs] on and those of sessions of length 0 are no tokens:
- * their q_out rows are left as they were.  Up to 2^24 - 1 tokens a call.  Pages shared between sessions
- * are read only: no two tokens of a call may come to stand in one slot. */
+ * their q_out rows are left as they were.  Up to 2^24 - 1 tokens a call.
+ * Pages shared between sessions are read only: no two tokens of a call may
+ * come to stand in one slot. */
 int c2h_paged_append_dev(c2h_ctx* ctx, const c2h_paged_kv* kv, const c2h_paged_batch* batch,
                          const int32_t* token_start, int32_t n_tokens, const c2h_rope* rope, int32_t type,
                          const c2h_heads* k, const c2h_heads* v, int32_t n_heads, const c2h_heads* q,
@@ -399,14 +400,20 @@ int c2h_paged_append_dev(c2h_ctx* ctx, const c2h_paged_kv* kv, const c2h_paged_b
  *   out = sum_j p_j v_j,  p = softmax_j(scale * q . k_j)
  * over the positions j < seq_lens[s] (the last `window` of them where
  * window > 0) of KV head h / (n_heads / n_kv_heads).  q and out are
- * [n_seqs][n_heads] vectors of `type` (F32, F16, BF16), up to 2^24 - 1 of them,
- * not overlapping.  A
- * session of length 0 gets zeros.  What a session holds is to be finite (a
- * NaN or an infinity there makes its head's rows NaN or infinite); what stands
- * elsewhere in the pool does not matter.  Scores, softmax and sums are 32-bit, the
- * result is rounded once to `type`; the same call on the same data gives the
- * same bits (how long sessions are split follows from the batch's lengths and
- * the descriptions alone).
+ * [n_seqs][n_heads] vectors of `type` (F32, F16, BF16), up to 2^24 - 1 of
+ * them, not overlapping.  A session of length 0 gets zeros.  What a session
+ * holds is to be finite (a NaN or an infinity there makes its head's rows NaN
+ * or infinite); what stands elsewhere in the pool does not matter.
+ * Sums of products, the softmax's maxima and sums, and the join are 32-bit,
+ * and the result is rounded once to `type`.  What the products take: over an
+ * F32 pool 32-bit numbers.  Over F16 and F8_E4M3 pools queries of F32 and the
+ * probabilities as 22 bits (two 16-bit parts), 16-bit queries as they are (an
+ * element below 2^-28 of its head's largest loses bits).  Over BF16 pools F32
+ * and F16 queries and their probabilities as 24 bits (three parts); BF16
+ * queries as they are, their probabilities at head_dim 64, 128 and 256 as 16
+ * bits (two parts, off by at most 2^-17) and else as 24.  The same call on the same data gives the same bits (how long
+ * sessions are split follows from the batch's lengths and the descriptions
+ * alone).
  * Work of several workgroups on one row meets in a workspace of the
  * context, which c2h_paged_attn_workspace sizes; it grows, with a wait for
  * the stream, in the first call that needs more than any before. */
@@ -419,7 +426,8 @@ int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* batc
                              size_t* bytes);
 
 /* RMSNorm with the residual's addition and Q8_K rows as its output: for each
- * of n_rows (up to 2^22 - 1) rows of cols elements (256 .. 16384) of `type` (F32, F16, BF16)
+ * of n_rows (up to 2^22 - 1) rows of cols elements (256 .. 16384) of `type`
+ * (F32, F16, BF16)
  *   s = x + residual (rounded to the type and stored to sum_out; s = x where
  *       residual is NULL),
  *   y = (s * f32(1 / sqrt(mean(s^2) + eps))) * w,
@@ -430,8 +438,9 @@ int c2h_paged_attn_workspace(const c2h_paged_kv* kv, const c2h_paged_batch* batc
  * formats whose products read f32 rows.  Rows of x, residual and sum_out are
  * x_stride, residual_stride and sum_stride elements apart, those of y_out
  * y_stride floats; any alignment of whole elements (q8k_out: 4 bytes), rows
- * and cols of multiples of four elements being the faster ones.  sum_out is required with a residual (NULL without) and may be x or
- * the residual itself (same pointer and stride). */
+ * and cols of multiples of four elements being the faster ones.  sum_out is
+ * required with a residual (NULL without) and may be x or the residual itself
+ * (same pointer and stride). */
 int c2h_rmsnorm_q8k_dev(c2h_ctx* ctx, int32_t type, const void* x, int64_t x_stride, const void* residual,
                         int64_t residual_stride, const float* w, float eps, int32_t n_rows, int32_t cols,
                         void* sum_out, int64_t sum_stride, void* q8k_out, float* y_out, int64_t y_stride);
